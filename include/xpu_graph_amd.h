@@ -438,6 +438,70 @@ int xg_rope(const void* x, const void* cos_table, const void* sin_table, void* o
             int table_dtype, xg_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Query / key preparation: rotary positions with one axis or several, and the
+ * per-head RMS norm in the same pass.
+ *   n = x rsqrt(mean(x^2) + eps) w           (xg_rope_axes: n = x; w NULL: 1)
+ *   pair i < R/2 of a row, R = rot_dim:  (n[i], n[i + R/2]) turns by row
+ *   positions[pair_axis[i], b, s] of the tables, rotate-half convention as in
+ *   xg_rope; elements from R on pass through.  fp32 math, one rounding.
+ * xg_rotary describes the rotation:
+ *   cos_table, sin_table: [table_rows, table_cols], row stride table_stride,
+ *     table_cols = R/2 (an entry per pair) or R (an entry per element: pair i
+ *     uses columns i and i + R/2), dtype table_dtype = `dtype` or XG_F32.
+ *   positions: DEVICE int32 / int64 (positions_64bit), element [a, b, s] at
+ *     pos_strides[0] a + pos_strides[1] b + pos_strides[2] s; or NULL (one axis
+ *     only): row s, or row 0 for every token when table_rows is 1.  A position
+ *     outside [0, table_rows) reads nothing outside the tables and gives NaN in
+ *     the elements it rotates.
+ *   axes <= 4; pair_axis: HOST array of R/2 axis numbers (NULL: one axis).
+ * x, q, k and their outputs are [B, heads, S, D] with element strides for
+ * batch, head, sequence and a unit last stride; strides multiples of 16 bytes;
+ * D % 16 == 0, D <= 512, R % 16 == 0, R <= D; dtype XG_BF16, XG_F16, XG_F32.
+ * At most 2^31 - 1 rows (B S heads).
+ *   xg_rope_axes: transpose != 0 applies the transposed rotation, which is the
+ *     gradient of x.
+ *   xg_qk_norm_rope: q [B,H,S,D] and k [B,Hkv,S,D] in one launch; either may
+ *     have no heads.  round_norm != 0 rounds n to `dtype` before the rotation,
+ *     as xg_rms_norm followed by xg_rope does (bit for bit in bf16 at D 64 and
+ *     128, where the kernels add a row up in the same order).
+ *   xg_qk_norm_rope_bwd: dq, dk from the upstream gradients gq, gk of the two
+ *     outputs, and gw_q, gw_k [D] (in w_dtype; NULL: not wanted), summed over
+ *     rows in a fixed order (no atomics) through a workspace of
+ *     xg_qk_norm_rope_bwd_workspace_floats fp32 (NULL when neither is wanted).
+ * No counterpart in the reference: what it leaves to eager before
+ *   aten.scaled_dot_product_attention
+ *   (passes/patterns/common/fuse_scaled_dot_product_attention.py:184-234).
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  const void* cos_table;
+  const void* sin_table;
+  int64_t table_rows;
+  int64_t table_cols;
+  int64_t table_stride;
+  int64_t rot_dim;
+  const void* positions;
+  int64_t pos_strides[3];
+  const uint8_t* pair_axis;
+  int32_t table_dtype;
+  int32_t positions_64bit;
+  int32_t axes;
+  int32_t pad;
+} xg_rotary;
+int xg_rope_axes(const void* x, void* out, int64_t B, int64_t H, int64_t S, int64_t D, const int64_t x_strides[3],
+                 const int64_t o_strides[3], const xg_rotary* rotary, int transpose, int dtype, xg_stream_t stream);
+int xg_qk_norm_rope(const void* q, const void* k, const void* q_w, const void* k_w, void* q_out, void* k_out, int64_t B,
+                    int64_t H, int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3], const int64_t k_strides[3],
+                    const int64_t qo_strides[3], const int64_t ko_strides[3], const xg_rotary* rotary, float eps,
+                    int round_norm, int dtype, int w_dtype, xg_stream_t stream);
+int64_t xg_qk_norm_rope_bwd_workspace_floats(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D);
+int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const void* k_w, const void* gq, const void* gk,
+                        void* dq, void* dk, void* gw_q, void* gw_k, float* workspace, int64_t workspace_floats, int64_t B,
+                        int64_t H, int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3],
+                        const int64_t k_strides[3], const int64_t gq_strides[3], const int64_t gk_strides[3],
+                        const int64_t dq_strides[3], const int64_t dk_strides[3], const xg_rotary* rotary, float eps,
+                        int dtype, int w_dtype, xg_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Plain device copy of `bytes` bytes (16-byte aligned), used as the known-size
  * yardstick that scales the FETCH_SIZE / WRITE_SIZE profiler counters.
  * ------------------------------------------------------------------------- */

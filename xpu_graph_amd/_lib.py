@@ -26,6 +26,14 @@ class XgChunk(ctypes.Structure):
     _fields_ = [("src_off", ctypes.c_int32), ("dst_off", ctypes.c_int32), ("out_id", ctypes.c_int32), ("pad", ctypes.c_int32)]
 
 
+class XgRotary(ctypes.Structure):
+    _fields_ = [
+        ("cos_table", c_void_p), ("sin_table", c_void_p), ("table_rows", c_int64), ("table_cols", c_int64), ("table_stride", c_int64),
+        ("rot_dim", c_int64), ("positions", c_void_p), ("pos_strides", c_int64 * 3), ("pair_axis", c_char_p), ("table_dtype", ctypes.c_int32),
+        ("positions_64bit", ctypes.c_int32), ("axes", ctypes.c_int32), ("pad", ctypes.c_int32),
+    ]
+
+
 class XgError(RuntimeError):
     """A C-ABI entry point refused its arguments or failed to launch."""
 
@@ -152,6 +160,16 @@ _SIGNATURES = {
     "xg_rope": (
         c_int,
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, ctypes.POINTER(c_int64), ctypes.POINTER(c_int64), c_int64, c_int, c_int, c_void_p],
+    ),
+    "xg_rope_axes": (c_int, [c_void_p] * 2 + [c_int64] * 4 + [ctypes.POINTER(c_int64)] * 2 + [ctypes.POINTER(XgRotary), c_int, c_int, c_void_p]),
+    "xg_qk_norm_rope": (
+        c_int,
+        [c_void_p] * 6 + [c_int64] * 5 + [ctypes.POINTER(c_int64)] * 4 + [ctypes.POINTER(XgRotary), c_float, c_int, c_int, c_int, c_void_p],
+    ),
+    "xg_qk_norm_rope_bwd_workspace_floats": (c_int64, [c_int64] * 5),
+    "xg_qk_norm_rope_bwd": (
+        c_int,
+        [c_void_p] * 11 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 6 + [ctypes.POINTER(XgRotary), c_float, c_int, c_int, c_void_p],
     ),
     "xg_copy_bytes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "xg_clock_probe": (c_int, [c_void_p, c_int, c_int64, c_void_p]),

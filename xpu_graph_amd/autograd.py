@@ -15,6 +15,9 @@ a few microseconds of dispatch, which inference-only processes should not pay.
     dense(x, W, trans, bias, residual, act)   y = act(x W(^T) + bias + residual)
     dense_glu(x, Wg, Wu)       y = silu(x Wg^T) * (x Wu^T)
     rope(x, cos, sin)          y = x * cos + rotate_half(x) * sin,  rotate_half(x) = cat(-x[D/2:], x[:D/2])
+    rope_axes(x, cos, sin, positions, ...)   the rotation with gathered positions (gradient: the transposed rotation)
+    qk_norm_rope(q, k, wq, wk, cos, sin, positions, ..., eps)   rotation of the per-head RMS norms of q and k (gradients: the fused
+                               xg_qk_norm_rope_bwd kernel; the tables of both ops get none)
     sdpa(q, k, v, causal, scale)   y = softmax(scale q k^T [+ causal mask]) v
     sdpa_lse(q, k, v, causal, scale)   the same, also returning the log-sum-exp of every row for the backward kernels
     sdpa_masked(q, k, v, mask, scale_t, causal, scale) / sdpa_masked_lse   with an additive mask and / or the scale in a
@@ -278,6 +281,40 @@ def _rope_backward(ctx, gy):
     return gx, gcos, gsin
 
 
+def _refuse_table_grad(ctx, name, cos):
+    if ctx.needs_input_grad[cos] or ctx.needs_input_grad[cos + 1]:
+        raise NotImplementedError(f"xpu_ops::{name}: no gradient for the cos / sin tables")
+
+
+def _rope_axes_setup(ctx, inputs, output):
+    _, cos, sin, positions, ctx.sections, ctx.interleaved = inputs
+    ctx.has_pos = positions is not None
+    ctx.save_for_backward(cos, sin, *((positions,) if ctx.has_pos else ()))
+
+
+def _rope_axes_backward(ctx, gy):
+    _refuse_table_grad(ctx, "rope_axes", 1)
+    cos, sin, *pos = ctx.saved_tensors
+    gx = torch.ops.xpu_ops.rope_axes_bwd(gy, cos, sin, pos[0] if pos else None, ctx.sections, ctx.interleaved) if ctx.needs_input_grad[0] else None
+    return gx, None, None, None, None, None
+
+
+def _qk_norm_rope_setup(ctx, inputs, output):
+    q, k, wq, wk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps, _ = inputs
+    ctx.has = [t is not None for t in (wq, wk, positions)]
+    ctx.save_for_backward(q, k, cos, sin, *(t for t in (wq, wk, positions) if t is not None))
+
+
+def _qk_norm_rope_backward(ctx, gq, gk):
+    _refuse_table_grad(ctx, "qk_norm_rope", 4)
+    q, k, cos, sin, *rest = ctx.saved_tensors
+    wq, wk, positions = (rest.pop(0) if has else None for has in ctx.has)
+    want_gw = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
+    dq, dk, gwq, gwk = torch.ops.xpu_ops.qk_norm_rope_bwd(q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps, want_gw)
+    need = ctx.needs_input_grad
+    return dq, dk, gwq if wq is not None and need[2] else None, gwk if wk is not None and need[3] else None, *((None,) * 7)
+
+
 def _sdpa_setup(ctx, inputs, output):
     q, k, v, ctx.causal, ctx.scale = inputs
     ctx.save_for_backward(q, k, v)
@@ -420,6 +457,8 @@ def register():
     reg("xpu_ops::dense_glu", _dense_glu_backward, setup_context=_dense_glu_setup)
     reg("xpu_ops::dense_glu_save", _dense_glu_save_backward, setup_context=_dense_glu_save_setup)
     reg("xpu_ops::rope", _rope_backward, setup_context=_rope_setup)
+    reg("xpu_ops::rope_axes", _rope_axes_backward, setup_context=_rope_axes_setup)
+    reg("xpu_ops::qk_norm_rope", _qk_norm_rope_backward, setup_context=_qk_norm_rope_setup)
     reg("xpu_ops::sdpa", _sdpa_backward, setup_context=_sdpa_setup)
     reg("xpu_ops::sdpa_lse", _sdpa_lse_backward, setup_context=_sdpa_lse_setup)
     reg("xpu_ops::sdpa_masked", _sdpa_masked_backward, setup_context=_sdpa_masked_setup)
@@ -430,7 +469,7 @@ def register():
         reg(f"xpu_ops::{op}", backward, setup_context=setup)
     # An op that was traced before (an inference compile earlier in the process) has its dispatch decisions cached
     # on the Python side; a stale entry for the Autograd key would keep sending traces to the "no formula" fallback.
-    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "sdpa", "sdpa_lse",
+    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "sdpa", "sdpa_lse",
                  "sdpa_masked", "sdpa_masked_lse", "add_rms_norm", "add_rms_norm_only", "add_layer_norm", "add_layer_norm_only"):
         packet = getattr(torch.ops.xpu_ops, name)
         for overload in packet.overloads():

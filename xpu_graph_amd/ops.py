@@ -11,6 +11,7 @@ Op names follow the reference's convention of a vendor op namespace allowed
 inside device graphs (`xpu_ops`, src/xpu_graph/backends/device_graph.py:26-29).
 """
 import ctypes
+import functools
 from typing import List, Optional
 
 import torch
@@ -1221,6 +1222,229 @@ _library.impl("sdpa_masked_bwd", _sdpa_masked_bwd, "CUDA")
 _library.impl("sdpa_masked_bwd", _sdpa_masked_bwd_meta, "Meta")
 _library.impl("rope", _rope, "CUDA")
 _library.impl("rope", _rope_meta, "Meta")
+
+
+# ------------------------------------------------ query / key preparation
+_library.define("rope_axes(Tensor x, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
+_library.define("rope_axes_bwd(Tensor gy, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
+_library.define(
+    "qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, Tensor? positions, int[] sections, "
+    "bool interleaved, float eps, bool round_norm=False) -> (Tensor, Tensor)"
+)
+_library.define(
+    "qk_norm_rope_bwd(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor gq, Tensor gk, Tensor cos, Tensor sin, Tensor? positions, "
+    "int[] sections, bool interleaved, float eps, bool want_gw) -> (Tensor, Tensor, Tensor, Tensor)"
+)
+
+ROPE_MAX_AXES = 4
+ROPE_MAX_HEAD_DIM = 512
+
+
+def _same_device(first, *others):
+    for t in others:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"xpu_ops: tensors on different devices ({first.device} and {t.device})")
+
+
+def _call(device, fn, what, *args):
+    """One launch on `device`'s current stream, whatever the current device is."""
+    index = device.index
+    if index == _current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    _lib.check(status, what)
+
+
+@functools.lru_cache(maxsize=256)
+def rope_pair_axes(sections, interleaved=False):
+    """The axis that turns each of the sum(sections) pairs of a row, as bytes.  In runs: the first sections[0] pairs belong
+    to axis 0, the next sections[1] to axis 1, ...; interleaved: pair i belongs to axis i % n while i < n * sections[i % n],
+    and to axis 0 from there on."""
+    n = len(sections)
+    if not interleaved:
+        return bytes(a for a, count in enumerate(sections) for _ in range(count))
+    return bytes(i % n if i < n * sections[i % n] else 0 for i in range(sum(sections)))
+
+
+def _rotary_check(x, cos, sin, positions, sections):
+    """Refuses what the rotation cannot take; returns (rotated columns, table columns, axes)."""
+    if x.dim() != 4:
+        raise ValueError("rope_axes: q, k or x must be [B, H, S, D]")
+    B, _, S, D = x.shape
+    if D % 16 != 0 or not 0 < D <= ROPE_MAX_HEAD_DIM:
+        raise ValueError(f"rope_axes: head dim must be a multiple of 16, at most {ROPE_MAX_HEAD_DIM}")
+    if cos.shape != sin.shape or cos.dim() < 1 or any(d != 1 for d in cos.shape[:-2]):
+        raise ValueError("rope_axes: cos / sin must be [P, R] or [P, R/2] tables of one shape (leading dims of size 1 allowed)")
+    if cos.dtype != sin.dtype or cos.dtype not in (x.dtype, torch.float32):
+        raise TypeError("rope_axes: cos / sin must share a dtype, that of x or float32")
+    cols = cos.shape[-1]
+    axes = len(sections) or 1
+    if axes > ROPE_MAX_AXES or any(n < 0 for n in sections):
+        raise ValueError(f"rope_axes: sections are the pairs of each axis, at most {ROPE_MAX_AXES} axes")
+    rot = 2 * sum(sections) if sections else D
+    if rot <= 0 or rot > D or rot % 16 != 0 or cols not in (rot, rot // 2):
+        raise ValueError("rope_axes: 2 * sum(sections) = R must be a multiple of 16 up to the head dim, the tables R or R/2 columns wide")
+    rows = cos.shape[-2] if cos.dim() > 1 else 1
+    if positions is None:
+        if axes != 1 or (rows != S and rows != 1):
+            raise ValueError("rope_axes: without positions there is one axis and the tables have one row per token, or one row")
+    else:
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError("rope_axes: positions must be int32 or int64")
+        shape = tuple(positions.shape)
+        full = (1,) * (3 - len(shape)) + shape
+        if len(shape) not in ((1, 2, 3) if axes == 1 else (3,)) or full[0] != axes or full[1] not in (1, B) or full[2] != S:
+            raise ValueError("rope_axes: positions must be [axes, B, S] ([S] or [B, S] with one axis; a batch dim of 1 is shared)")
+        if rows == 0:
+            raise ValueError("rope_axes: the tables are empty")
+    return rot, cols, axes
+
+
+def _table_2d(t, cols):
+    per16 = 16 // t.element_size()
+    t = t.reshape(-1, cols)
+    return t if t.stride(1) == 1 and t.stride(0) >= cols and t.stride(0) % per16 == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+
+
+def _rotary(x, cos, sin, positions, sections, interleaved):
+    """The xg_rotary of a call and what it points to."""
+    rot, cols, axes = _rotary_check(x, cos, sin, positions, sections)
+    _same_device(x, cos, sin, positions)
+    cos, sin = _table_2d(cos, cols), _table_2d(sin, cols)
+    if cos.stride(0) != sin.stride(0):
+        cos, sin = cos.contiguous(), sin.contiguous()
+    if cos.data_ptr() % 16 or sin.data_ptr() % 16 or (cols * cos.element_size()) % 16 and cos.shape[0] > 1:
+        raise ValueError("rope_axes: rows of the tables must be multiples of 16 bytes")
+    r = _lib.XgRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], cols, max(cos.stride(0), cols), rot)
+    r.table_dtype, r.axes = _code(cos.dtype), axes
+    if positions is not None:
+        r.positions, r.positions_64bit = positions.data_ptr(), int(positions.dtype == torch.int64)
+        strides = (0,) * (3 - positions.dim()) + positions.stride()
+        r.pos_strides[0], r.pos_strides[2] = strides[0], strides[2]
+        r.pos_strides[1] = strides[1] if positions.dim() > 1 and positions.shape[-2] > 1 else 0
+    if axes > 1:
+        r.pair_axis = rope_pair_axes(tuple(sections), bool(interleaved))
+    return r, (cos, sin)
+
+
+def _rope_axes_run(x, cos, sin, positions, sections, interleaved, transpose):
+    code = _code(x.dtype)
+    r, _keep = _rotary(x, cos, sin, positions, sections, interleaved)
+    x = _unit_last(x)
+    out = _empty_like_layout(x)
+    if out.numel():
+        S3 = ctypes.c_int64 * 3
+        _call(x.device, _lib.lib().xg_rope_axes, "xg_rope_axes", _ptr(x), _ptr(out), *x.shape, S3(*x.stride()[:3]), S3(*out.stride()[:3]), r,
+              transpose, code)
+    return out
+
+
+def _rope_axes(x, cos, sin, positions, sections, interleaved=False):
+    """Rotary positions with several axes: pair i of a row turns by row positions[axis of i, b, s] of the tables (see
+    rope_pair_axes); columns from R = 2 * sum(sections) on pass through.  Without sections: one axis, R = D."""
+    return _rope_axes_run(x, cos, sin, positions, sections, interleaved, 0)
+
+
+def _rope_axes_bwd(gy, cos, sin, positions, sections, interleaved=False):
+    """The gradient of x: the transposed rotation of gy."""
+    return _rope_axes_run(gy, cos, sin, positions, sections, interleaved, 1)
+
+
+def _rope_axes_meta(x, cos, sin, positions, sections, interleaved=False):
+    _rotary_check(x, cos, sin, positions, sections)
+    return _empty_like_layout(_unit_last(x))
+
+
+def _qk_check(q, k, q_weight, k_weight):
+    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
+        raise ValueError("qk_norm_rope: q and k must be [B, H, S, D] and [B, Hkv, S, D]")
+    if q.dtype != k.dtype:
+        raise TypeError("qk_norm_rope: q and k must share a dtype")
+    for w in (q_weight, k_weight):
+        if w is not None and tuple(w.shape) != (q.shape[3],):
+            raise ValueError("qk_norm_rope: a weight is one row of the head dim")
+
+
+def _qk_weights(q, q_weight, k_weight):
+    (q_weight, k_weight), w_dtype = _param_dtype(q.dtype, q_weight, k_weight)
+    # the kernel reads 16 bytes at a time; a weight that is a slice of a larger tensor may start anywhere
+    q_weight, k_weight = (w.clone() if w is not None and w.data_ptr() % 16 else w for w in (q_weight, k_weight))
+    return q_weight, k_weight, w_dtype
+
+
+def _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps, round_norm=False):
+    """RMS norm over each head of q and of k and the rotation of rope_axes, in one launch for both.  round_norm rounds the
+    normalised rows to the tensors' dtype before they turn, as rms_norm followed by rope does."""
+    _qk_check(q, k, q_weight, k_weight)
+    code = _code(q.dtype)
+    _same_device(q, k, q_weight, k_weight)
+    r, _keep = _rotary(q, cos, sin, positions, sections, interleaved)
+    q, k = _unit_last(q), _unit_last(k)
+    q_out, k_out = _empty_like_layout(q), _empty_like_layout(k)
+    if q_out.numel() + k_out.numel():
+        q_weight, k_weight, w_dtype = _qk_weights(q, q_weight, k_weight)
+        B, H, S, D = q.shape
+        S3 = ctypes.c_int64 * 3
+        _call(q.device, _lib.lib().xg_qk_norm_rope, "xg_qk_norm_rope", _ptr(q), _ptr(k), _ptr(q_weight), _ptr(k_weight), _ptr(q_out), _ptr(k_out),
+              B, H, k.shape[1], S, D, S3(*q.stride()[:3]), S3(*k.stride()[:3]), S3(*q_out.stride()[:3]), S3(*k_out.stride()[:3]), r, eps,
+              1 if round_norm else 0, code, _code(w_dtype))
+    return q_out, k_out
+
+
+def _qk_norm_rope_meta(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps, round_norm=False):
+    _qk_check(q, k, q_weight, k_weight)
+    _rotary_check(q, cos, sin, positions, sections)
+    return _empty_like_layout(_unit_last(q)), _empty_like_layout(_unit_last(k))
+
+
+def _qk_norm_rope_bwd(q, k, q_weight, k_weight, gq, gk, cos, sin, positions, sections, interleaved, eps, want_gw):
+    """(dq, dk, gw_q, gw_k) for the upstream gradients of the two outputs; the weight gradients are empty when not wanted
+    or without a weight."""
+    _qk_check(q, k, q_weight, k_weight)
+    if gq.shape != q.shape or gk.shape != k.shape or gq.dtype != q.dtype or gk.dtype != q.dtype:
+        raise ValueError("qk_norm_rope_bwd: gq and gk must match q and k in shape and dtype")
+    code = _code(q.dtype)
+    _same_device(q, k, q_weight, k_weight, gq, gk)
+    r, _keep = _rotary(q, cos, sin, positions, sections, interleaved)
+    q, k, gq, gk = (_unit_last(t) for t in (q, k, gq, gk))
+    dq, dk = _empty_like_layout(q), _empty_like_layout(k)
+    gws = [torch.empty(w.shape, dtype=w.dtype, device=q.device) if want_gw and w is not None else None for w in (q_weight, k_weight)]
+    if dq.numel() + dk.numel() == 0:
+        gws = [g.zero_() if g is not None else None for g in gws]
+    else:
+        wq, wk, w_dtype = _qk_weights(q, q_weight, k_weight)
+        kernel_gws = [torch.empty_like(g, dtype=w_dtype) if g is not None and g.dtype != w_dtype else g for g in gws]
+        B, H, S, D = q.shape
+        Hkv = k.shape[1]
+        lib = _lib.lib()
+        n_ws = lib.xg_qk_norm_rope_bwd_workspace_floats(B, H, Hkv, S, D) if any(g is not None for g in gws) else 0
+        ws = torch.empty((n_ws,), dtype=torch.float32, device=q.device) if n_ws else None
+        S3 = ctypes.c_int64 * 3
+        _call(q.device, lib.xg_qk_norm_rope_bwd, "xg_qk_norm_rope_bwd", _ptr(q), _ptr(k), _ptr(wq), _ptr(wk), _ptr(gq), _ptr(gk), _ptr(dq), _ptr(dk),
+              _ptr(kernel_gws[0]), _ptr(kernel_gws[1]), _ptr(ws), n_ws, B, H, Hkv, S, D, *(S3(*t.stride()[:3]) for t in (q, k, gq, gk, dq, dk)), r, eps,
+              code, _code(w_dtype))
+        gws = [a if a is b else a.copy_(b) for a, b in zip(gws, kernel_gws)]
+    none = torch.empty(0, dtype=q.dtype, device=q.device)
+    return dq, dk, none if gws[0] is None else gws[0], none.clone() if gws[1] is None else gws[1]
+
+
+def _qk_norm_rope_bwd_meta(q, k, q_weight, k_weight, gq, gk, cos, sin, positions, sections, interleaved, eps, want_gw):
+    _qk_check(q, k, q_weight, k_weight)
+    none = lambda: torch.empty(0, dtype=q.dtype, device=q.device)  # noqa: E731
+    gws = [torch.empty(w.shape, dtype=w.dtype, device=q.device) if want_gw and w is not None else none() for w in (q_weight, k_weight)]
+    return (*(_empty_like_layout(_unit_last(t)) for t in (q, k)), *gws)
+
+
+_library.impl("rope_axes", _rope_axes, "CUDA")
+_library.impl("rope_axes", _rope_axes_meta, "Meta")
+_library.impl("rope_axes_bwd", _rope_axes_bwd, "CUDA")
+_library.impl("rope_axes_bwd", _rope_axes_meta, "Meta")
+_library.impl("qk_norm_rope", _qk_norm_rope, "CUDA")
+_library.impl("qk_norm_rope", _qk_norm_rope_meta, "Meta")
+_library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd, "CUDA")
+_library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd_meta, "Meta")
 
 
 # ------------------------------------------------------------- training
