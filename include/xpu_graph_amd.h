@@ -502,6 +502,57 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
                         int dtype, int w_dtype, xg_stream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Linear attention with a decay for each head:
+ *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+ * q, out [B,H,S,D], k, v [B,Hkv,S,D] (query head h reads head h / (H / Hkv));
+ * strides in elements for batch, head, sequence, multiples of 8, unit last
+ * stride; D in {64, 128}; XG_BF16 or XG_F16.  log_decay: DEVICE fp32 [H], at
+ * most 0 in a model (minus infinity: no memory).
+ * States are fp32 [B,H,D,D] contiguous (row: k, column: v), 16-byte aligned.
+ *   state: before the first token, or NULL (zeros); state_out: after the last,
+ *     or NULL.
+ *   lengths: NULL, or DEVICE int32 / int64 [B] (lengths_64bit), clamped to
+ *     [0, S]: tokens from there on are not read, do not reach the state, and
+ *     give zeros in out and in the gradients.
+ *   A NaN or an infinity in q, k or v reaches the outputs of its own chunk of
+ *   64 tokens and of all later tokens.
+ * xg_linear_attn: a whole sequence, 64 tokens at a time on the matrix cores.
+ *   Up to three launches; workspace: xg_linear_attn_workspace_floats fp32 (0:
+ *   none needed).
+ * xg_linear_attn_bwd: dq, dk, dv (own strides, as the gradients of xg_sdpa)
+ *   and d_state (NULL: not wanted) from d_out and d_state_out (NULL: none).
+ *   log_decay gets no gradient.  Sums in a fixed order, no atomics; the
+ *   gradients of shared heads are added up in fp32.  workspace:
+ *   xg_linear_attn_bwd_workspace_floats fp32.
+ * xg_linear_attn_step: one token; `state` is updated in place.  q, k, v, out:
+ *   strides of batch and head, any alignment; state_strides: batch and head,
+ *   multiples of 4, the [D,D] matrices contiguous; states that overlap are
+ *   refused.
+ * No counterpart in the reference: the sibling of its
+ *   aten.scaled_dot_product_attention pattern
+ *   (passes/patterns/common/fuse_scaled_dot_product_attention.py:184-234) for
+ *   models whose attention keeps a state instead of keys and values.
+ * ------------------------------------------------------------------------- */
+int64_t xg_linear_attn_workspace_floats(int64_t B, int64_t H, int64_t S, int64_t D);
+int xg_linear_attn(const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                   const void* lengths, int lengths_64bit, void* out, float* state_out, float* workspace,
+                   int64_t workspace_floats, int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D,
+                   const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                   const int64_t o_strides[3], float scale, int dtype, xg_stream_t stream);
+int64_t xg_linear_attn_bwd_workspace_floats(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D);
+int xg_linear_attn_bwd(const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                       const void* lengths, int lengths_64bit, const void* d_out, const float* d_state_out, void* dq,
+                       void* dk, void* dv, float* d_state, float* workspace, int64_t workspace_floats, int64_t B,
+                       int64_t H, int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3],
+                       const int64_t k_strides[3], const int64_t v_strides[3], const int64_t do_strides[3],
+                       const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
+                       float scale, int dtype, xg_stream_t stream);
+int xg_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, void* out,
+                        int64_t B, int64_t H, int64_t Hkv, int64_t D, const int64_t q_strides[2],
+                        const int64_t k_strides[2], const int64_t v_strides[2], const int64_t o_strides[2],
+                        const int64_t state_strides[2], float scale, int dtype, xg_stream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Plain device copy of `bytes` bytes (16-byte aligned), used as the known-size
  * yardstick that scales the FETCH_SIZE / WRITE_SIZE profiler counters.
  * ------------------------------------------------------------------------- */

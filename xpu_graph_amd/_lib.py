@@ -171,6 +171,17 @@ _SIGNATURES = {
         c_int,
         [c_void_p] * 11 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 6 + [ctypes.POINTER(XgRotary), c_float, c_int, c_int, c_void_p],
     ),
+    "xg_linear_attn_workspace_floats": (c_int64, [c_int64] * 4),
+    "xg_linear_attn": (
+        c_int,
+        [c_void_p] * 6 + [c_int] + [c_void_p] * 3 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 4 + [c_float, c_int, c_void_p],
+    ),
+    "xg_linear_attn_bwd_workspace_floats": (c_int64, [c_int64] * 5),
+    "xg_linear_attn_bwd": (
+        c_int,
+        [c_void_p] * 6 + [c_int] + [c_void_p] * 7 + [c_int64] * 6 + [ctypes.POINTER(c_int64)] * 7 + [c_float, c_int, c_void_p],
+    ),
+    "xg_linear_attn_step": (c_int, [c_void_p] * 6 + [c_int64] * 4 + [ctypes.POINTER(c_int64)] * 5 + [c_float, c_int, c_void_p]),
     "xg_copy_bytes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "xg_clock_probe": (c_int, [c_void_p, c_int, c_int64, c_void_p]),
     "xg_wall_clock_khz": (c_int64, []),

@@ -18,6 +18,8 @@ a few microseconds of dispatch, which inference-only processes should not pay.
     rope_axes(x, cos, sin, positions, ...)   the rotation with gathered positions (gradient: the transposed rotation)
     qk_norm_rope(q, k, wq, wk, cos, sin, positions, ..., eps)   rotation of the per-head RMS norms of q and k (gradients: the fused
                                xg_qk_norm_rope_bwd kernel; the tables of both ops get none)
+    linear_attn(q, k, v, log_decay, state, lengths, scale)   y_t = scale q_t S_t, S_t = exp(log_decay) S_{t-1} + k_t v_t^T (gradients: the
+                               same kernel with the operands in other roles, xg_linear_attn_bwd; log_decay gets none)
     sdpa(q, k, v, causal, scale)   y = softmax(scale q k^T [+ causal mask]) v
     sdpa_lse(q, k, v, causal, scale)   the same, also returning the log-sum-exp of every row for the backward kernels
     sdpa_masked(q, k, v, mask, scale_t, causal, scale) / sdpa_masked_lse   with an additive mask and / or the scale in a
@@ -315,6 +317,27 @@ def _qk_norm_rope_backward(ctx, gq, gk):
     return dq, dk, gwq if wq is not None and need[2] else None, gwk if wk is not None and need[3] else None, *((None,) * 7)
 
 
+def _linear_attn_setup(ctx, inputs, output):
+    q, k, v, log_decay, state, lengths, ctx.scale = inputs
+    ctx.has = [t is not None for t in (state, lengths)]
+    ctx.save_for_backward(q, k, v, log_decay, *(t for t in (state, lengths) if t is not None))
+    ctx.set_materialize_grads(False)  # an unused output hands over None: no gradient of the final state is read then
+
+
+def _linear_attn_backward(ctx, gy, g_state=None):
+    if ctx.needs_input_grad[3]:
+        raise NotImplementedError("xpu_ops::linear_attn: no gradient for log_decay (only q, k, v and the state are differentiable)")
+    if gy is None and g_state is None:
+        return (None,) * 7
+    q, k, v, log_decay, *rest = ctx.saved_tensors
+    state, lengths = (rest.pop(0) if has else None for has in ctx.has)
+    if gy is None:
+        gy = torch.zeros_like(q)
+    want_d_state = state is not None and ctx.needs_input_grad[4]
+    dq, dk, dv, d_state = torch.ops.xpu_ops.linear_attn_bwd(q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want_d_state)
+    return dq, dk, dv, None, d_state if want_d_state else None, None, None
+
+
 def _sdpa_setup(ctx, inputs, output):
     q, k, v, ctx.causal, ctx.scale = inputs
     ctx.save_for_backward(q, k, v)
@@ -459,6 +482,7 @@ def register():
     reg("xpu_ops::rope", _rope_backward, setup_context=_rope_setup)
     reg("xpu_ops::rope_axes", _rope_axes_backward, setup_context=_rope_axes_setup)
     reg("xpu_ops::qk_norm_rope", _qk_norm_rope_backward, setup_context=_qk_norm_rope_setup)
+    reg("xpu_ops::linear_attn", _linear_attn_backward, setup_context=_linear_attn_setup)
     reg("xpu_ops::sdpa", _sdpa_backward, setup_context=_sdpa_setup)
     reg("xpu_ops::sdpa_lse", _sdpa_lse_backward, setup_context=_sdpa_lse_setup)
     reg("xpu_ops::sdpa_masked", _sdpa_masked_backward, setup_context=_sdpa_masked_setup)
@@ -469,7 +493,7 @@ def register():
         reg(f"xpu_ops::{op}", backward, setup_context=setup)
     # An op that was traced before (an inference compile earlier in the process) has its dispatch decisions cached
     # on the Python side; a stale entry for the Autograd key would keep sending traces to the "no formula" fallback.
-    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "sdpa", "sdpa_lse",
+    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "linear_attn", "sdpa", "sdpa_lse",
                  "sdpa_masked", "sdpa_masked_lse", "add_rms_norm", "add_rms_norm_only", "add_layer_norm", "add_layer_norm_only"):
         packet = getattr(torch.ops.xpu_ops, name)
         for overload in packet.overloads():

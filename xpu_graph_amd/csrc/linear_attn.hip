@@ -1,0 +1,868 @@
+// Linear attention with a decay for each head, for gfx950:
+//
+//   S_t = lam S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   lam = exp(log_decay[h]),   S a [D, D] matrix per head in fp32
+//
+// Chunked form, 64 tokens at a time; S the state before the chunk, n its tokens, i and j rows in it:
+//   P[i][j] = (q_i . k_j) lam^(i-j)   for j <= i, else 0
+//   o_i     = scale (sum_j P[i][j] v_j + lam^(i+1) q_i S)
+//   S'      = lam^n S + sum_j lam^(n-1-j) k_j v_j^T
+//
+// Its gradients are the same recurrence with the operands in other roles (F: the forward form, F_rev: the tokens backwards):
+//   dq = scale F(do, v, k), state S^T;   dv = F_rev(k, q, do), dk = F_rev(v, do, q), state G = scale sum lam^(t-s) q_t do_t^T
+// In F_rev the incoming gradient of the final state enters undecayed, so its state is kept one decay ahead (e = 1 below), and
+// what it ends with is the gradient of the initial state.
+//
+// One kernel serves all of them (Problem says which operand is which).  A workgroup owns one head of one batch entry and a
+// segment of its tokens; wave w owns the 16 columns 16w..16w+15 of S in its accumulators, where they stay in fp32 from chunk to
+// chunk, and computes those columns of O.  The products are transposed (O^T = S^T Q^T + V^T P^T), so that S goes from
+// accumulator to operand without leaving the lane: the k index of an MFMA may be permuted as long as both operands agree, and
+// the order used throughout is the one the accumulators hold.  P passes through LDS, since every wave needs all of it.
+//
+// Roundings to 16 bits: S and P where they are operands of the product that gives O, as the scores of any tiled attention are
+// (one rounding each, against the one of O itself).  The state is an fp32 result, and it is carried over the whole sequence, so
+// there lam^(n-1-j) v_j is split into three bf16 parts, which hold its 24 bits.  fp16 tensors have three more bits than bf16
+// and a range that neither S nor P fits, so their operands are split into bf16 parts as well: two each for q, k, v (exact), S
+// and P, and products of the small parts are left out.
+//
+// A few heads do not fill the chip.  The tokens are then cut into segments: one launch sums up each segment's own state, one
+// turns them into the states before each segment (elementwise, in order), and the kernel above runs all segments at once.
+#include "sdpa_common.hpp"
+
+namespace xg {
+namespace linattn {
+
+using sdpa::lds_s16x4;
+using sdpa::s16x4;
+using sdpa::s16x8;
+using sdpa::static_for;
+using sdpa::swz_v;
+using sdpa::Vec8;
+
+constexpr int C = 64;         // tokens per chunk
+constexpr int P_ROW = 160;    // bytes per query row of P in LDS: 64 keys and a pad that spreads eight rows over the banks
+constexpr float kLog2e = 1.44269504088896340736f;
+
+struct Operand {
+  const void* p;
+  int64_t s[3];  // element strides of batch, head, token
+  int group;     // query heads per head of this tensor
+};
+
+struct Problem {
+  Operand q, k, v;
+  void* out;
+  int64_t os[3];
+  int out_f32;              // out is fp32 (shares of shared heads), else the tensors' type
+  const float* state0;      // [B, H, D, D] or NULL (zeros)
+  float* state_out;         // [B, H, D, D] or NULL
+  float* seg_states;        // [B H][n_seg][D D] in accumulator order (n_seg > 1)
+  int state0_t;             // state0 is read transposed
+  int reverse;
+  int e;                    // the state is kept e decays ahead
+  float s_intra, s_inter, s_state;
+};
+
+struct Params {
+  Problem pr[3];
+  const float* log_decay;
+  const void* lengths;      // [B] or NULL
+  int len64;
+  int B, H, S;
+  int n_seg, seg_chunks;
+};
+
+__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// A value in N bf16 parts, largest first.
+template <int N>
+struct Parts {
+  bf16x8 v[N];
+};
+template <int N>
+__device__ __forceinline__ Parts<N> split(const float (&x)[8]) {
+  Parts<N> p;
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = x[i];
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p.v[k][i] = (bf16_t)r[i];
+    if (k + 1 < N) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] -= (float)p.v[k][i];
+    }
+  }
+  return p;
+}
+
+// An operand of the products that give O: one bf16 part for bf16 tensors, two for fp16.
+template <typename T>
+constexpr int kParts = std::is_same_v<T, f16_t> ? 2 : 1;
+
+template <typename T>
+__device__ __forceinline__ Parts<kParts<T>> as_parts(typename Vec8<T>::type x) {
+  if constexpr (kParts<T> == 1) {
+    return Parts<1>{{x}};
+  } else {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)x[i];
+    return split<2>(f);
+  }
+}
+
+// Sum of the products of two split operands; parts i and j meet while i + j < max(NA, NB).
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mma_parts(const Parts<NA>& a, const Parts<NB>& b, f32x4 c) {
+  constexpr int N = NA > NB ? NA : NB;
+#pragma unroll
+  for (int i = NA - 1; i >= 0; --i)
+#pragma unroll
+    for (int j = NB - 1; j >= 0; --j)
+      if (i + j < N) c = mma16(a.v[i], b.v[j], c);
+  return c;
+}
+
+__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+template <typename T, int D>
+struct Tile {
+  static constexpr int RB = D * 2;
+  static constexpr int BYTES = C * RB;
+  typedef typename Vec8<T>::type V8;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+
+  // row `row`, columns 32 kk + 8 q4 .. +7
+  __device__ static __forceinline__ V8 row_frag(const char* tile, int row, int kk, int q4) {
+    return *reinterpret_cast<const V8*>(tile + row * RB + (((4 * kk + q4) ^ swz_v<D>(row)) << 4));
+  }
+  // row `row`, columns 32 t + 4 q4 .. +3 and 32 t + 16 + 4 q4 .. +3
+  __device__ static __forceinline__ V8 row_frag_perm(const char* tile, int row, int t, int q4) {
+    const int sub = (q4 & 1) << 3, ch = 4 * t + (q4 >> 1);
+    const T4 lo = *reinterpret_cast<const T4*>(tile + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub);
+    const T4 hi = *reinterpret_cast<const T4*>(tile + row * RB + (((ch + 2) ^ swz_v<D>(row)) << 4) + sub);
+    return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  }
+  // column 16 ct + a16, rows 32 t + 4 q4 .. +3 and 32 t + 16 + 4 q4 .. +3 (two transposing reads)
+  __device__ static __forceinline__ V8 col_frag(const char* tile, int ct, int t, int q4, int a16) {
+    const int row = 32 * t + 4 * q4 + (a16 >> 2), ch = 2 * ct + ((a16 & 3) >> 1), sub = (a16 & 1) << 3;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (row + 16) * RB + ((ch ^ swz_v<D>(row + 16)) << 4) + sub));
+    const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    return __builtin_bit_cast(V8, both);
+  }
+};
+
+__device__ __forceinline__ int length_of(const Params& p, int b) {
+  if (!p.lengths) return p.S;
+  const int64_t n = p.len64 ? reinterpret_cast<const int64_t*>(p.lengths)[b] : (int64_t) reinterpret_cast<const int32_t*>(p.lengths)[b];
+  return n < 0 ? 0 : (n > p.S ? p.S : (int)n);
+}
+
+// lam^n for whole n >= 0; a decay of minus infinity gives 1, 0, 0, ...
+__device__ __forceinline__ float head_log2(const Params& p, int h) {
+  const float g = p.log_decay[h] * kLog2e;
+  return g < -1e30f ? -1e30f : g;
+}
+__device__ __forceinline__ float decay(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
+
+// The rows of one operand's chunk on their way from global memory to LDS.
+template <typename T, int D>
+struct Mover {
+  static constexpr int NT = D * 4;            // threads: D/16 waves
+  static constexpr int N = C * D / 8 / NT;    // 16-byte pieces per thread
+  const char* base;
+  int64_t row_bytes;                          // signed: a reversed operand walks backwards
+  u32x4 piece[N];
+
+  __device__ __forceinline__ void bind(const Operand& o, int b, int h, int len, int reverse) {
+    const int64_t last = reverse ? (int64_t)(len - 1) * o.s[2] : 0;
+    base = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (h / o.group) * o.s[1] + last) * 2;
+    row_bytes = (reverse ? -o.s[2] : o.s[2]) * 2;
+  }
+  __device__ __forceinline__ void load(int t0, int end, int tid) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = i * NT + tid, row = idx / (D / 8), c = idx % (D / 8);
+      piece[i] = u32x4{0, 0, 0, 0};
+      if (t0 + row < end) piece[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)(t0 + row) * row_bytes + c * 16);
+    }
+  }
+  __device__ __forceinline__ void store(char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int idx = i * NT + tid, row = idx / (D / 8), c = idx % (D / 8);
+      *reinterpret_cast<u32x4*>(tile + row * (D * 2) + ((c ^ swz_v<D>(row)) << 4)) = piece[i];
+    }
+  }
+};
+
+// S' = lam^n S + sum_j f_j k_j v_j^T on this wave's 16 columns; f[t][jj] belongs to the token of slot jj of k-step t.
+template <typename T, int D>
+__device__ __forceinline__ void update_state(f32x4 (&S)[D / 16], const char* k_tile, const typename Vec8<T>::type (&vf)[2], const float (&f)[2][8],
+                                             float lam_n, int q4, int a16) {
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) S[dt] *= lam_n;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    float x[8];
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj) x[jj] = (float)vf[t][jj] * f[t][jj];
+    const Parts<3> fv = split<3>(x);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) S[dt] = mma_parts(as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, q4, a16)), fv, S[dt]);
+  }
+}
+
+__device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n, int e, float s_state, int q4) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int jj = 0; jj < 8; ++jj) {
+      const int left = n - 1 - (32 * t + 4 * q4 + (jj & 3) + (jj < 4 ? 0 : 16));
+      f[t][jj] = decay(g2, left < 0 ? 0 : left + e) * s_state;
+    }
+}
+
+// Each segment's own state (from zero), in accumulator order.
+template <typename T, int D>
+__global__ __launch_bounds__(D * 4) void segment_states_kernel(const Params p) {
+  __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<T, D>::BYTES];
+  char* k_s = smem;
+  char* v_s = smem + Tile<T, D>::BYTES;
+  const Problem& pr = p.pr[blockIdx.y];
+  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, a16 = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
+  const int b = bh / p.H, h = bh % p.H;
+  const int len = length_of(p, b);
+  const int t_beg = seg * p.seg_chunks * C;
+  const int t_end = t_beg + p.seg_chunks * C < len ? t_beg + p.seg_chunks * C : len;
+  if (t_beg >= t_end) return;
+  const float g2 = head_log2(p, h);
+  f32x4 S[D / 16];
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  Mover<T, D> km, vm;
+  km.bind(pr.k, b, h, len, pr.reverse);
+  vm.bind(pr.v, b, h, len, pr.reverse);
+  float f[2][8];
+  token_factors(f, g2, C, pr.e, pr.s_state, q4);
+  km.load(t_beg, t_end, tid);
+  vm.load(t_beg, t_end, tid);
+  for (int t0 = t_beg; t0 < t_end; t0 += C) {
+    const int n = t_end - t0 < C ? t_end - t0 : C;
+    if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, q4);
+    lds_barrier();
+    km.store(k_s, tid);
+    vm.store(v_s, tid);
+    lds_barrier();
+    if (t0 + C < t_end) {
+      km.load(t0 + C, t_end, tid);
+      vm.load(t0 + C, t_end, tid);
+    }
+    typename Vec8<T>::type vf[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) vf[t] = Tile<T, D>::col_frag(v_s, w, t, q4, a16);
+    update_state<T, D>(S, k_s, vf, f, decay(g2, n), q4, a16);
+  }
+  float* to = pr.seg_states + (int64_t)blockIdx.x * (D * D);
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(to + ((w * (D / 16) + dt) * 64 + lane) * 4) = S[dt];
+}
+
+// Segment states in order: what segment m added becomes the state before segment m.  One thread per four elements.
+template <int D>
+__global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
+  const Problem& pr = p.pr[blockIdx.y];
+  constexpr int PER = D * D / 1024;  // blocks per head
+  const int bh = blockIdx.x / PER;
+  const int at = (blockIdx.x % PER) * 1024 + threadIdx.x * 4;
+  const int b = bh / p.H, h = bh % p.H;
+  const int lane = (at >> 2) & 63, dt = (at >> 8) % (D / 16), w = (at >> 8) / (D / 16);
+  const int dk = 16 * dt + 4 * (lane >> 4), dv = 16 * w + (lane & 15);
+  const int len = length_of(p, b);
+  const float g2 = head_log2(p, h);
+  f32x4 S = {0.f, 0.f, 0.f, 0.f};
+  if (pr.state0) {
+    const float* s0 = pr.state0 + (int64_t)bh * (D * D);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) S[r] = pr.state0_t ? s0[dv * D + dk + r] : s0[(dk + r) * D + dv];
+  }
+  float* ws = pr.seg_states + (int64_t)bh * p.n_seg * (D * D) + at;
+  const int seg_len = p.seg_chunks * C;
+  for (int m = 0; m < p.n_seg; ++m) {
+    const int left = len - m * seg_len;
+    const int n = left < 0 ? 0 : (left < seg_len ? left : seg_len);
+    f32x4* cell = reinterpret_cast<f32x4*>(ws + (int64_t)m * (D * D));
+    if (n == 0) break;  // no segment from here on has tokens
+    const f32x4 own = *cell;
+    *cell = S;
+    S = S * decay(g2, n) + own;
+  }
+  if (pr.state_out) {
+    float* so = pr.state_out + (int64_t)bh * (D * D);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) so[(dk + r) * D + dv] = S[r];
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(D * 4) void linear_attn_kernel(const Params p) {
+  typedef typename Vec8<T>::type V8;
+  typedef Tile<T, D> TL;
+  constexpr int NW = D / 16;                       // waves
+  constexpr int NP = (10 + NW - 1) / NW;           // tiles of P per wave (10 of the 4 x 4 lie on or below the diagonal)
+  constexpr int PP = kParts<T>;
+  extern __shared__ __attribute__((aligned(1024))) char smem[];
+  char* q_s = smem;
+  char* k_s = smem + TL::BYTES;
+  char* v_s = smem + 2 * TL::BYTES;
+  char* p_s = smem + 3 * TL::BYTES;                // [PP][64 queries][P_ROW bytes]
+  const Problem& pr = p.pr[blockIdx.y];
+  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, a16 = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
+  const int b = bh / p.H, h = bh % p.H;
+  const int len = length_of(p, b);
+  const int t_beg = seg * p.seg_chunks * C;
+  const int s_end = t_beg + p.seg_chunks * C < p.S ? t_beg + p.seg_chunks * C : p.S;
+  const int t_end = s_end < len ? s_end : len;
+  const float g2 = head_log2(p, h);
+
+  // rows behind the sequence: zeros
+  {
+    const int from = t_beg > len ? t_beg : len;
+    const int64_t row0 = b * pr.os[0] + h * pr.os[1];
+    for (int idx = tid; idx < (s_end - from) * (D / 8); idx += D * 4) {
+      const int64_t at = row0 + (int64_t)(from + idx / (D / 8)) * pr.os[2] + (idx % (D / 8)) * 8;
+      const u32x4 zero = {0, 0, 0, 0};
+      if (pr.out_f32) {
+        u32x4* o = reinterpret_cast<u32x4*>(reinterpret_cast<float*>(pr.out) + at);
+        o[0] = zero;
+        o[1] = zero;
+      } else {
+        *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(pr.out) + at) = zero;
+      }
+    }
+  }
+
+  // the state before the segment
+  f32x4 S[D / 16];
+#pragma unroll
+  for (int dt = 0; dt < D / 16; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if (p.n_seg > 1) {
+    if (t_beg >= t_end) return;
+    const float* from = pr.seg_states + (int64_t)blockIdx.x * (D * D);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt) S[dt] = *reinterpret_cast<const f32x4*>(from + ((w * (D / 16) + dt) * 64 + lane) * 4);
+  } else if (pr.state0) {
+    const float* s0 = pr.state0 + (int64_t)bh * (D * D);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int dk = 16 * dt + 4 * q4 + r, dv = 16 * w + a16;
+        S[dt][r] = pr.state0_t ? s0[dv * D + dk] : s0[dk * D + dv];
+      }
+  }
+  const bool keep_state = p.n_seg == 1 && pr.state_out;
+
+  if (t_beg < t_end) {
+    Mover<T, D> qm, km, vm;
+    qm.bind(pr.q, b, h, len, pr.reverse);
+    km.bind(pr.k, b, h, len, pr.reverse);
+    vm.bind(pr.v, b, h, len, pr.reverse);
+    qm.load(t_beg, t_end, tid);
+    km.load(t_beg, t_end, tid);
+    vm.load(t_beg, t_end, tid);
+
+    // factors that do not change from chunk to chunk
+    float f[2][8];
+    token_factors(f, g2, C, pr.e, pr.s_state, q4);
+    float row_f[4];
+#pragma unroll
+    for (int qt = 0; qt < 4; ++qt) row_f[qt] = decay(g2, 16 * qt + a16 + 1 - pr.e) * pr.s_inter;
+    float p_f[NP][4];
+    int p_kt[NP], p_qt[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const int id = w + NW * i;
+      p_qt[i] = id >= 6 ? 3 : (id >= 3 ? 2 : (id >= 1 ? 1 : 0));
+      p_kt[i] = id - p_qt[i] * (p_qt[i] + 1) / 2;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int d = 16 * (p_qt[i] - p_kt[i]) + a16 - 4 * q4 - r;
+        p_f[i][r] = d < 0 ? 0.f : decay(g2, d) * pr.s_intra;
+      }
+    }
+    // the two tiles of P above the diagonal that the 32-key steps read: always zero
+    for (int idx = tid; idx < PP * 2 * 16 * 2; idx += D * 4) {
+      const int half = idx & 1, row = (idx >> 1) & 15, which = (idx >> 5) & 1, part = idx >> 6;
+      *reinterpret_cast<u32x4*>(p_s + part * C * P_ROW + (32 * which + row) * P_ROW + (32 * which + 16) * 2 + half * 16) = u32x4{0, 0, 0, 0};
+    }
+
+    for (int t0 = t_beg; t0 < t_end; t0 += C) {
+      const int n = t_end - t0 < C ? t_end - t0 : C;
+      lds_barrier();  // every wave is done with the previous chunk's tiles
+      qm.store(q_s, tid);
+      km.store(k_s, tid);
+      vm.store(v_s, tid);
+      lds_barrier();
+      if (t0 + C < t_end) {
+        qm.load(t0 + C, t_end, tid);
+        km.load(t0 + C, t_end, tid);
+        vm.load(t0 + C, t_end, tid);
+      }
+
+      // P^T = K Q^T, decayed
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        if (w + NW * i < 10) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int kk = 0; kk < D / 32; ++kk)
+            acc = mma16(TL::row_frag(k_s, 16 * p_kt[i] + a16, kk, q4), TL::row_frag(q_s, 16 * p_qt[i] + a16, kk, q4), acc);
+          char* to = p_s + (16 * p_qt[i] + a16) * P_ROW + (16 * p_kt[i] + 4 * q4) * 2;
+          float x[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) x[r] = 16 * (p_qt[i] - p_kt[i]) + a16 - 4 * q4 - r >= 0 ? acc[r] * p_f[i][r] : 0.f;
+#pragma unroll
+          for (int part = 0; part < PP; ++part) {
+            bf16x4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              y[r] = (bf16_t)x[r];
+              x[r] -= (float)y[r];
+            }
+            *reinterpret_cast<bf16x4*>(to + part * C * P_ROW) = y;
+          }
+        }
+      }
+
+      // O^T = S^T Q^T, each query scaled by its decay
+      f32x4 O[4];
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) O[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) {
+        float x[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) x[r] = S[2 * t][r], x[4 + r] = S[2 * t + 1][r];
+        const Parts<PP> sp = split<PP>(x);
+#pragma unroll
+        for (int qt = 0; qt < 4; ++qt) O[qt] = mma_parts(sp, as_parts<T>(TL::row_frag_perm(q_s, 16 * qt + a16, t, q4)), O[qt]);
+      }
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) O[qt] *= row_f[qt];
+      V8 vf[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(v_s, w, t, q4, a16);
+      lds_barrier();  // P is whole
+
+      // O^T += V^T P^T
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const Parts<PP> vp = as_parts<T>(vf[t]);
+#pragma unroll
+        for (int qt = 2 * t; qt < 4; ++qt) {
+          Parts<PP> pp;
+#pragma unroll
+          for (int part = 0; part < PP; ++part) {
+            const char* row = p_s + part * C * P_ROW + (16 * qt + a16) * P_ROW + (32 * t + 4 * q4) * 2;
+            const bf16x4 lo = *reinterpret_cast<const bf16x4*>(row), hi = *reinterpret_cast<const bf16x4*>(row + 32);
+            pp.v[part] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          }
+          O[qt] = mma_parts(vp, pp, O[qt]);
+        }
+      }
+
+      // lane: query 16 qt + a16, columns 16 w + 4 q4 .. +3
+#pragma unroll
+      for (int qt = 0; qt < 4; ++qt) {
+        const int row = 16 * qt + a16;
+        if (row < n) {
+          const int64_t token = pr.reverse ? (int64_t)len - 1 - (t0 + row) : (int64_t)t0 + row;
+          const int64_t at = b * pr.os[0] + h * pr.os[1] + token * pr.os[2] + 16 * w + 4 * q4;
+          if (pr.out_f32) {
+            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(pr.out) + at) = O[qt];
+          } else {
+            typename TL::T4 y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = (T)O[qt][r];
+            *reinterpret_cast<typename TL::T4*>(reinterpret_cast<T*>(pr.out) + at) = y;
+          }
+        }
+      }
+
+      if (t0 + C < t_end || keep_state) {
+        if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, q4);
+        update_state<T, D>(S, k_s, vf, f, decay(g2, n), q4, a16);
+      }
+    }
+  }
+
+  if (keep_state) {
+    float* so = pr.state_out + (int64_t)bh * (D * D);
+#pragma unroll
+    for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) so[(16 * dt + 4 * q4 + r) * D + 16 * w + a16] = S[dt][r];
+  }
+}
+
+// Shared heads: the gradient of a key / value head is the sum over its query heads, in their order.  part: [B, H, S, D] fp32.
+struct GroupSum {
+  const float* part[2];
+  void* out[2];
+  int64_t os[2][3];
+  int64_t n;      // B * Hkv * S * D / 4
+  int Hkv, S, D, group;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void group_sum_kernel(const GroupSum p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= p.n) return;
+  const int per_row = p.D / 4;
+  const int c = (int)(i % per_row) * 4;
+  const int64_t row = i / per_row;
+  const int s = (int)(row % p.S);
+  const int hk = (int)((row / p.S) % p.Hkv);
+  const int64_t b = row / ((int64_t)p.S * p.Hkv);
+  const float* src = p.part[blockIdx.y] + (((b * p.Hkv + hk) * p.group) * p.S + s) * (int64_t)p.D + c;
+  f32x4 a = *reinterpret_cast<const f32x4*>(src);
+  for (int g = 1; g < p.group; ++g) a += *reinterpret_cast<const f32x4*>(src + (int64_t)g * p.S * p.D);
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 y;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = (T)a[r];
+  const int64_t* os = p.os[blockIdx.y];
+  *reinterpret_cast<T4*>(reinterpret_cast<T*>(p.out[blockIdx.y]) + b * os[0] + hk * os[1] + s * os[2] + c) = y;
+}
+
+// One token: the state of a head is read, updated and written in place, and the row q S comes out of the same pass.
+// Bound by the state's bytes (two ways).  A workgroup takes 32 columns of one head's state: eight lanes per row (16 bytes each,
+// 128-byte lines), 32 rows at a time.
+struct StepParams {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  float* state;
+  const float* log_decay;
+  int64_t qs[2], ks[2], vs[2], os[2], ss[2];  // batch, head
+  int H, group;
+  float scale;
+};
+template <typename T, int D>
+__global__ __launch_bounds__(256) void linear_attn_step_kernel(const StepParams p) {
+  __shared__ f32x4 red[4][8];
+  const int tid = threadIdx.x, c = (tid & 7) * 4, r0 = tid >> 3;
+  const int part = blockIdx.x % (D / 32), bh = blockIdx.x / (D / 32);
+  const int64_t b = bh / p.H;
+  const int h = bh % p.H, hk = h / p.group;
+  const int col = 32 * part + c;
+  float* st = p.state + b * p.ss[0] + h * p.ss[1] + col;
+  f32x4 S[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) S[i] = *reinterpret_cast<const f32x4*>(st + (int64_t)(r0 + 32 * i) * D);
+  const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1];
+  const T* k = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[1];
+  const T* v = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[1] + col;
+  const float lam = expf(p.log_decay[h]);
+  f32x4 vv, acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int r = 0; r < 4; ++r) vv[r] = to_f32(v[r]);
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    const float kr = to_f32(k[r0 + 32 * i]), qr = to_f32(q[r0 + 32 * i]);
+    S[i] = S[i] * lam + kr * vv;
+    *reinterpret_cast<f32x4*>(st + (int64_t)(r0 + 32 * i) * D) = S[i];
+    acc += qr * S[i];
+  }
+#pragma unroll
+  for (int off = 8; off < 64; off <<= 1)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] += __shfl_xor(acc[r], off, kWave);
+  if ((tid & 63) < 8) red[tid >> 6][tid & 7] = acc;
+  __syncthreads();
+  if (tid < 8) {
+    f32x4 t = red[0][tid];
+#pragma unroll
+    for (int i = 1; i < 4; ++i) t += red[i][tid];
+    T* o = reinterpret_cast<T*>(p.out) + b * p.os[0] + h * p.os[1] + col;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = from_f32<T>(t[r] * p.scale);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
+
+// How many segments the tokens of a head are cut into: enough workgroups to fill the chip twice over, at least two chunks each.
+void segments(int64_t heads, int64_t S, int& n_seg, int& seg_chunks) {
+  const int64_t chunks = chunks_of(S);
+  int64_t n = (512 + heads - 1) / heads;
+  if (n > chunks / 2) n = chunks / 2;
+  if (n < 1) n = 1;
+  seg_chunks = (int)((chunks + n - 1) / n);
+  n_seg = (int)((chunks + seg_chunks - 1) / seg_chunks);
+}
+
+int check(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D, float scale, int dtype) {
+  if (dtype != XG_BF16 && dtype != XG_F16) return XG_ERR_BAD_DTYPE;
+  if (B < 0 || H < 0 || Hkv < 0 || S < 0 || (D != 64 && D != 128)) return XG_ERR_BAD_SHAPE;
+  if (B && H && (Hkv == 0 || H % Hkv != 0)) return XG_ERR_BAD_SHAPE;
+  if (!(scale == scale) || fabsf(scale) > 3.0e38f) return XG_ERR_BAD_ARG;
+  if (S > (1 << 30) || B > (1 << 24) || H > (1 << 24) || B * H > (1 << 20)) return XG_ERR_TOO_LARGE;
+  return XG_OK;
+}
+
+int fill(int64_t (&to)[3], const int64_t* from) {
+  if (!from) return XG_ERR_NULL_PTR;
+  for (int i = 0; i < 3; ++i) {
+    if (from[i] < 0) return XG_ERR_BAD_SHAPE;
+    if (from[i] % 8) return XG_ERR_BAD_ALIGN;
+    to[i] = from[i];
+  }
+  return XG_OK;
+}
+
+int fill(Operand& o, const void* p, const int64_t* s, int group) {
+  if (!p) return XG_ERR_NULL_PTR;
+  if (!aligned_to(p, 16)) return XG_ERR_BAD_ALIGN;
+  o.p = p;
+  o.group = group;
+  return fill(o.s, s);
+}
+
+template <typename T, int D>
+int launch(const Params& p, int n_problems, hipStream_t st) {
+  constexpr int SMEM = 3 * Tile<T, D>::BYTES + kParts<T> * C * P_ROW;
+  auto kernel = linear_attn_kernel<T, D>;
+  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), SMEM)) return rc;
+  const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems);
+  if (p.n_seg > 1) {
+    hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, dim3(D * 4), 0, st, p);
+    hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
+  }
+  hipLaunchKernelGGL(kernel, grid, dim3(D * 4), SMEM, st, p);
+  return status_from_hip(hipGetLastError());
+}
+
+int launch_any(const Params& p, int n_problems, int64_t D, int dtype, hipStream_t st) {
+  if (dtype == XG_BF16) return D == 64 ? launch<bf16_t, 64>(p, n_problems, st) : launch<bf16_t, 128>(p, n_problems, st);
+  return D == 64 ? launch<f16_t, 64>(p, n_problems, st) : launch<f16_t, 128>(p, n_problems, st);
+}
+
+}  // namespace linattn
+}  // namespace xg
+
+extern "C" int64_t xg_linear_attn_workspace_floats(int64_t B, int64_t H, int64_t S, int64_t D) {
+  using namespace xg::linattn;
+  if (check(B, H, H, S, D, 1.f, XG_BF16) != XG_OK || B == 0 || H == 0 || S == 0) return 0;
+  int n_seg, seg_chunks;
+  segments(B * H, S, n_seg, seg_chunks);
+  return n_seg > 1 ? B * H * n_seg * D * D : 0;
+}
+
+extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const float* log_decay, const float* state, const void* lengths,
+                              int lengths_64bit, void* out, float* state_out, float* workspace, int64_t workspace_floats, int64_t B, int64_t H,
+                              int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3], const int64_t k_strides[3],
+                              const int64_t v_strides[3], const int64_t o_strides[3], float scale, int dtype, xg_stream_t stream) {
+  using namespace xg;
+  using namespace xg::linattn;
+  if (int rc = check(B, H, Hkv, S, D, scale, dtype)) return rc;
+  if (B == 0 || H == 0 || S == 0) return XG_OK;
+  if (!log_decay || !out) return XG_ERR_NULL_PTR;
+  if (!aligned_to(out, 16) || !aligned_to(log_decay, 4) || (state && !aligned_to(state, 16)) || (state_out && !aligned_to(state_out, 16)) ||
+      (workspace && !aligned_to(workspace, 16)) || (lengths && !aligned_to(lengths, lengths_64bit ? 8 : 4)))
+    return XG_ERR_BAD_ALIGN;
+  Params p{};
+  const int group = (int)(H / Hkv);
+  if (int rc = fill(p.pr[0].q, q, q_strides, 1)) return rc;
+  if (int rc = fill(p.pr[0].k, k, k_strides, group)) return rc;
+  if (int rc = fill(p.pr[0].v, v, v_strides, group)) return rc;
+  if (int rc = fill(p.pr[0].os, o_strides)) return rc;
+  p.log_decay = log_decay;
+  p.lengths = lengths;
+  p.len64 = lengths_64bit != 0;
+  p.B = (int)B;
+  p.H = (int)H;
+  p.S = (int)S;
+  segments(B * H, S, p.n_seg, p.seg_chunks);
+  if (p.n_seg > 1) {
+    if (!workspace) return XG_ERR_NULL_PTR;
+    if (workspace_floats < B * H * p.n_seg * D * D) return XG_ERR_BAD_ARG;
+  }
+  Problem& pr = p.pr[0];
+  pr.out = out;
+  pr.state0 = state;
+  pr.state_out = state_out;
+  pr.seg_states = workspace;
+  pr.s_intra = pr.s_inter = scale;
+  pr.s_state = 1.f;
+  return launch_any(p, 1, D, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+extern "C" int64_t xg_linear_attn_bwd_workspace_floats(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D) {
+  using namespace xg::linattn;
+  if (check(B, H, Hkv, S, D, 1.f, XG_BF16) != XG_OK || B == 0 || H == 0 || S == 0) return 0;
+  return 3 * xg_linear_attn_workspace_floats(B, H, S, D) + (H != Hkv ? 2 * B * H * S * D : 0);
+}
+
+extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, const float* log_decay, const float* state, const void* lengths,
+                                  int lengths_64bit, const void* d_out, const float* d_state_out, void* dq, void* dk, void* dv, float* d_state,
+                                  float* workspace, int64_t workspace_floats, int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D,
+                                  const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                                  const int64_t do_strides[3], const int64_t dq_strides[3], const int64_t dk_strides[3],
+                                  const int64_t dv_strides[3], float scale, int dtype, xg_stream_t stream) {
+  using namespace xg;
+  using namespace xg::linattn;
+  if (int rc = check(B, H, Hkv, S, D, scale, dtype)) return rc;
+  if (B == 0 || H == 0 || S == 0) return XG_OK;
+  if (!log_decay || !dq || !dk || !dv) return XG_ERR_NULL_PTR;
+  for (const void* t : {(const void*)dq, (const void*)dk, (const void*)dv, (const void*)state, (const void*)d_state_out, (const void*)d_state,
+                        (const void*)workspace})
+    if (t && !aligned_to(t, 16)) return XG_ERR_BAD_ALIGN;
+  if (!aligned_to(log_decay, 4) || (lengths && !aligned_to(lengths, lengths_64bit ? 8 : 4))) return XG_ERR_BAD_ALIGN;
+  Params p{};
+  const int group = (int)(H / Hkv);
+  Operand oq, ok, ov, og;
+  if (int rc = fill(oq, q, q_strides, 1)) return rc;
+  if (int rc = fill(ok, k, k_strides, group)) return rc;
+  if (int rc = fill(ov, v, v_strides, group)) return rc;
+  if (int rc = fill(og, d_out, do_strides, 1)) return rc;
+  p.log_decay = log_decay;
+  p.lengths = lengths;
+  p.len64 = lengths_64bit != 0;
+  p.B = (int)B;
+  p.H = (int)H;
+  p.S = (int)S;
+  segments(B * H, S, p.n_seg, p.seg_chunks);
+  const int64_t need = xg_linear_attn_bwd_workspace_floats(B, H, Hkv, S, D);
+  if (need) {
+    if (!workspace) return XG_ERR_NULL_PTR;
+    if (workspace_floats < need) return XG_ERR_BAD_ARG;
+  }
+  const int64_t seg_floats = p.n_seg > 1 ? B * H * p.n_seg * D * D : 0;
+  float* partial = workspace + 3 * seg_floats;
+  // dq = scale F(do, v, k), its state the transpose of the forward's
+  Problem& a = p.pr[0];
+  a.q = og;
+  a.k = ov;
+  a.v = ok;
+  a.out = dq;
+  if (int rc = fill(a.os, dq_strides)) return rc;
+  a.state0 = state;
+  a.state0_t = 1;
+  a.s_intra = a.s_inter = scale;
+  a.s_state = 1.f;
+  // dv = F_rev(k, q, do): its state ends as the gradient of the initial state
+  Problem& c = p.pr[1];
+  c.q = ok;
+  c.k = oq;
+  c.v = og;
+  c.out = dv;
+  if (int rc = fill(c.os, dv_strides)) return rc;
+  c.state0 = d_state_out;
+  c.state_out = d_state;
+  // dk = F_rev(v, do, q): the transposed state
+  Problem& d = p.pr[2];
+  d.q = ov;
+  d.k = og;
+  d.v = oq;
+  d.out = dk;
+  if (int rc = fill(d.os, dk_strides)) return rc;
+  d.state0 = d_state_out;
+  d.state0_t = 1;
+  for (Problem* r : {&c, &d}) {
+    r->reverse = r->e = 1;
+    r->s_intra = r->s_state = scale;
+    r->s_inter = 1.f;
+  }
+  for (int i = 0; i < 3; ++i) p.pr[i].seg_states = workspace + i * seg_floats;
+  GroupSum gs{};
+  if (group > 1) {
+    for (int i = 0; i < 2; ++i) {
+      Problem& r = p.pr[1 + i];
+      gs.part[i] = partial + i * B * H * S * D;
+      gs.out[i] = r.out;
+      for (int j = 0; j < 3; ++j) gs.os[i][j] = r.os[j];
+      r.out = partial + i * B * H * S * D;
+      r.os[0] = H * S * D;
+      r.os[1] = S * D;
+      r.os[2] = D;
+      r.out_f32 = 1;
+    }
+    gs.n = B * Hkv * S * D / 4;
+    gs.Hkv = (int)Hkv;
+    gs.S = (int)S;
+    gs.D = (int)D;
+    gs.group = group;
+    if ((gs.n + 255) / 256 > 0x7fffffffLL) return XG_ERR_TOO_LARGE;
+  }
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (int rc = launch_any(p, 3, D, dtype, st)) return rc;
+  if (group > 1) {
+    const dim3 grid((unsigned)((gs.n + 255) / 256), 2);
+    if (dtype == XG_BF16)
+      hipLaunchKernelGGL((group_sum_kernel<bf16_t>), grid, dim3(256), 0, st, gs);
+    else
+      hipLaunchKernelGGL((group_sum_kernel<f16_t>), grid, dim3(256), 0, st, gs);
+  }
+  return status_from_hip(hipGetLastError());
+}
+
+extern "C" int xg_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, void* out, int64_t B,
+                                   int64_t H, int64_t Hkv, int64_t D, const int64_t q_strides[2], const int64_t k_strides[2],
+                                   const int64_t v_strides[2], const int64_t o_strides[2], const int64_t state_strides[2], float scale,
+                                   int dtype, xg_stream_t stream) {
+  using namespace xg;
+  using namespace xg::linattn;
+  if (int rc = check(B, H, Hkv, 1, D, scale, dtype)) return rc;
+  if (B == 0 || H == 0) return XG_OK;
+  if (!q || !k || !v || !log_decay || !state || !out || !q_strides || !k_strides || !v_strides || !o_strides || !state_strides)
+    return XG_ERR_NULL_PTR;
+  if (!aligned_to(q, 2) || !aligned_to(k, 2) || !aligned_to(v, 2) || !aligned_to(out, 2) || !aligned_to(state, 16) || !aligned_to(log_decay, 4))
+    return XG_ERR_BAD_ALIGN;
+  StepParams p;
+  for (int i = 0; i < 2; ++i) {
+    if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0 || o_strides[i] < 0 || state_strides[i] < 0) return XG_ERR_BAD_SHAPE;
+    if (state_strides[i] % 4) return XG_ERR_BAD_ALIGN;
+    p.qs[i] = q_strides[i];
+    p.ks[i] = k_strides[i];
+    p.vs[i] = v_strides[i];
+    p.os[i] = o_strides[i];
+    p.ss[i] = state_strides[i];
+  }
+  // states that overlap would be updated by several workgroups at once
+  const int64_t inner = D * D, s0 = state_strides[0], s1 = state_strides[1];
+  if ((H > 1 && s1 < inner) || (B > 1 && s0 < inner) || (B > 1 && H > 1 && s0 < (H - 1) * s1 + inner && s1 < (B - 1) * s0 + inner))
+    return XG_ERR_BAD_SHAPE;
+  p.q = q;
+  p.k = k;
+  p.v = v;
+  p.out = out;
+  p.state = state;
+  p.log_decay = log_decay;
+  p.H = (int)H;
+  p.group = (int)(H / Hkv);
+  p.scale = scale;
+  const dim3 grid((unsigned)(B * H * (D / 32)));
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (dtype == XG_BF16) {
+    if (D == 64)
+      hipLaunchKernelGGL((linear_attn_step_kernel<bf16_t, 64>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((linear_attn_step_kernel<bf16_t, 128>), grid, dim3(256), 0, st, p);
+  } else {
+    if (D == 64)
+      hipLaunchKernelGGL((linear_attn_step_kernel<f16_t, 64>), grid, dim3(256), 0, st, p);
+    else
+      hipLaunchKernelGGL((linear_attn_step_kernel<f16_t, 128>), grid, dim3(256), 0, st, p);
+  }
+  return status_from_hip(hipGetLastError());
+}

@@ -1447,6 +1447,155 @@ _library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd, "CUDA")
 _library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd_meta, "Meta")
 
 
+# ------------------------------------------------------- linear attention
+_library.define(
+    "linear_attn(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? state, Tensor? lengths, float scale) -> (Tensor, Tensor)"
+)
+_library.define(
+    "linear_attn_bwd(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? state, Tensor? lengths, Tensor d_out, Tensor? d_state_out, "
+    "float scale, bool want_d_state) -> (Tensor, Tensor, Tensor, Tensor)"
+)
+_library.define("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor(a!) state, float scale) -> Tensor")
+
+
+def _linear_attn_check(q, k, v, log_decay, state, lengths=None):
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("linear_attn: q must be [B, H, S, D], k and v [B, Hkv, S, D]")
+    B, H, S, D = q.shape
+    if k.shape[0] != B or k.shape[2:] != q.shape[2:] or H % max(k.shape[1], 1) != 0 or (k.shape[1] == 0) != (H == 0):
+        raise ValueError("linear_attn: inconsistent q/k/v shapes")
+    if D not in (64, 128):
+        raise ValueError("linear_attn: head dim must be 64 or 128")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("linear_attn: q, k, v must share a dtype, bfloat16 or float16")
+    if tuple(log_decay.shape) != (H,) or log_decay.dtype != torch.float32:
+        raise ValueError("linear_attn: log_decay must be float32 [H]")
+    if state is not None and (tuple(state.shape) != (B, H, D, D) or state.dtype != torch.float32):
+        raise ValueError("linear_attn: states must be float32 [B, H, D, D]")
+    if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
+        raise ValueError("linear_attn: lengths must be int32 or int64 [B]")
+    _same_device(q, k, v, log_decay, state, lengths)
+
+
+def _state_operand(state):
+    if state is None:
+        return None
+    state = state.contiguous()
+    return state.clone() if state.data_ptr() % 16 else state
+
+
+def _workspace(floats, device):
+    return torch.empty((floats,), dtype=torch.float32, device=device) if floats > 0 else None
+
+
+def _linear_attn(q, k, v, log_decay, state, lengths, scale):
+    """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t over a sequence: (out, the state after each entry's last
+    token).  state: the one before the first token (zeros without); lengths [B]: tokens from there on are not read, give zeros
+    and do not reach the state."""
+    _linear_attn_check(q, k, v, log_decay, state, lengths)
+    q, k, v = _unit_last(q), _unit_last(k), _unit_last(v)
+    B, H, S, D = q.shape
+    out = _empty_like_layout(q)
+    state_out = torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
+    if out.numel() == 0:
+        return out, (state_out.zero_() if state is None else state_out.copy_(state))
+    state, log_decay = _state_operand(state), log_decay.contiguous()
+    lengths = lengths.contiguous() if lengths is not None else None
+    lib = _lib.lib()
+    n_ws = lib.xg_linear_attn_workspace_floats(B, H, S, D)
+    ws = _workspace(n_ws, q.device)
+    S3 = ctypes.c_int64 * 3
+    _call(q.device, lib.xg_linear_attn, "xg_linear_attn", _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(lengths),
+          int(lengths is not None and lengths.dtype == torch.int64), _ptr(out), _ptr(state_out), _ptr(ws), n_ws, B, H, k.shape[1], S, D,
+          *(S3(*t.stride()[:3]) for t in (q, k, v, out)), scale, _code(q.dtype))
+    return out, state_out
+
+
+def _linear_attn_meta(q, k, v, log_decay, state, lengths, scale):
+    _linear_attn_check(q, k, v, log_decay, state, lengths)
+    B, H, _, D = q.shape
+    return _empty_like_layout(_unit_last(q)), torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
+
+
+def _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out):
+    _linear_attn_check(q, k, v, log_decay, state, lengths)
+    if d_out.shape != q.shape or d_out.dtype != q.dtype:
+        raise ValueError("linear_attn_bwd: d_out must match q in shape and dtype")
+    B, H, _, D = q.shape
+    if d_state_out is not None and (tuple(d_state_out.shape) != (B, H, D, D) or d_state_out.dtype != torch.float32):
+        raise ValueError("linear_attn_bwd: d_state_out must be float32 [B, H, D, D]")
+    _same_device(q, d_out, d_state_out)
+
+
+def _linear_attn_bwd(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
+    """(dq, dk, dv, d_state): the gradients of linear_attn's inputs from those of its two outputs (d_state_out may be None);
+    d_state is empty when not wanted.  log_decay gets none."""
+    _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out)
+    q, k, v, d_out = (_unit_last(t) for t in (q, k, v, d_out))
+    B, H, S, D = q.shape
+    dq, dk, dv = _empty_like_layout(q), _empty_like_layout(k), _empty_like_layout(v)
+    d_state = torch.empty((B, H, D, D) if want_d_state else (0,), dtype=torch.float32, device=q.device)
+    if dq.numel() == 0:
+        if want_d_state:
+            d_state.zero_() if d_state_out is None else d_state.copy_(d_state_out)
+        return dq, dk, dv, d_state
+    state, d_state_out, log_decay = _state_operand(state), _state_operand(d_state_out), log_decay.contiguous()
+    lengths = lengths.contiguous() if lengths is not None else None
+    lib = _lib.lib()
+    n_ws = lib.xg_linear_attn_bwd_workspace_floats(B, H, k.shape[1], S, D)
+    ws = _workspace(n_ws, q.device)
+    S3 = ctypes.c_int64 * 3
+    _call(q.device, lib.xg_linear_attn_bwd, "xg_linear_attn_bwd", _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(lengths),
+          int(lengths is not None and lengths.dtype == torch.int64), _ptr(d_out), _ptr(d_state_out), _ptr(dq), _ptr(dk), _ptr(dv),
+          _ptr(d_state) if want_d_state else None, _ptr(ws), n_ws, B, H, k.shape[1], S, D,
+          *(S3(*t.stride()[:3]) for t in (q, k, v, d_out, dq, dk, dv)), scale, _code(q.dtype))
+    return dq, dk, dv, d_state
+
+
+def _linear_attn_bwd_meta(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
+    _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out)
+    B, H, _, D = q.shape
+    d_state = torch.empty((B, H, D, D) if want_d_state else (0,), dtype=torch.float32, device=q.device)
+    return (*(_empty_like_layout(_unit_last(t)) for t in (q, k, v)), d_state)
+
+
+def _linear_attn_step_check(q, k, v, log_decay, state):
+    _linear_attn_check(q, k, v, log_decay, state)
+    if q.shape[2] != 1:
+        raise ValueError("linear_attn_step: one token, q [B, H, 1, D]")
+    D = q.shape[3]
+    if state.numel() and (state.stride(3) != 1 or state.stride(2) != D):
+        raise ValueError("linear_attn_step: the [D, D] matrices of the state must be contiguous (it is updated in place)")
+
+
+def _linear_attn_step(q, k, v, log_decay, state, scale):
+    """One token of linear_attn: the state is updated in place, the output row comes out of the same pass."""
+    _linear_attn_step_check(q, k, v, log_decay, state)
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    log_decay = log_decay.contiguous()
+    S2 = ctypes.c_int64 * 2
+    B, H, _, D = q.shape
+    _call(q.device, _lib.lib().xg_linear_attn_step, "xg_linear_attn_step", _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(out), B, H,
+          k.shape[1], D, *(S2(*t.stride()[:2]) for t in (q, k, v, out, state)), scale, _code(q.dtype))
+    return out
+
+
+def _linear_attn_step_meta(q, k, v, log_decay, state, scale):
+    _linear_attn_step_check(q, k, v, log_decay, state)
+    return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+
+_library.impl("linear_attn", _linear_attn, "CUDA")
+_library.impl("linear_attn", _linear_attn_meta, "Meta")
+_library.impl("linear_attn_bwd", _linear_attn_bwd, "CUDA")
+_library.impl("linear_attn_bwd", _linear_attn_bwd_meta, "Meta")
+_library.impl("linear_attn_step", _linear_attn_step, "CUDA")
+_library.impl("linear_attn_step", _linear_attn_step_meta, "Meta")
+
+
 # ------------------------------------------------------------- training
 def enable_autograd():
     """Register the backward formulas of the ops that may appear in training graphs (xpu_graph_amd/autograd.py).
