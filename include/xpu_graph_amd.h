@@ -505,8 +505,8 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  * Linear attention with a decay for each head:
  *   S_t = exp(log_decay[h]) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
  * q, out [B,H,S,D], k, v [B,Hkv,S,D] (query head h reads head h / (H / Hkv));
- * strides in elements for batch, head, sequence, multiples of 8, unit last
- * stride; D in {64, 128}; XG_BF16 or XG_F16.  log_decay: DEVICE fp32 [H], at
+ * strides in elements for batch, head, sequence, multiples of 8 (below 2^26
+ * for the sequence), unit last stride; D in {64, 128}; XG_BF16 or XG_F16.  log_decay: DEVICE fp32 [H], at
  * most 0 in a model (minus infinity: no memory).
  * States are fp32 [B,H,D,D] contiguous (row: k, column: v), 16-byte aligned.
  *   state: before the first token, or NULL (zeros); state_out: after the last,
@@ -515,8 +515,8 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  *     [0, S]: tokens from there on are not read, do not reach the state, and
  *     give zeros in out and in the gradients.
  *   A NaN or an infinity in q, k or v reaches the outputs of its own chunk of
- *   64 tokens and of all later tokens.
- * xg_linear_attn: a whole sequence, 64 tokens at a time on the matrix cores.
+ *   32 tokens and of all later tokens.
+ * xg_linear_attn: a whole sequence, 32 tokens at a time on the matrix cores.
  *   Up to three launches; workspace: xg_linear_attn_workspace_floats fp32 (0:
  *   none needed).
  * xg_linear_attn_bwd: dq, dk, dv (own strides, as the gradients of xg_sdpa)

@@ -2,7 +2,7 @@
 //
 //   S_t = lam S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,   lam = exp(log_decay[h]),   S a [D, D] matrix per head in fp32
 //
-// Chunked form, 64 tokens at a time; S the state before the chunk, n its tokens, i and j rows in it:
+// Chunked form, 32 tokens at a time; S the state before the chunk, n its tokens, i and j rows in it:
 //   P[i][j] = (q_i . k_j) lam^(i-j)   for j <= i, else 0
 //   o_i     = scale (sum_j P[i][j] v_j + lam^(i+1) q_i S)
 //   S'      = lam^n S + sum_j lam^(n-1-j) k_j v_j^T
@@ -13,16 +13,20 @@
 // what it ends with is the gradient of the initial state.
 //
 // One kernel serves all of them (Problem says which operand is which).  A workgroup owns one head of one batch entry and a
-// segment of its tokens; wave w owns the 16 columns 16w..16w+15 of S in its accumulators, where they stay in fp32 from chunk to
-// chunk, and computes those columns of O.  The products are transposed (O^T = S^T Q^T + V^T P^T), so that S goes from
+// segment of its tokens; wave w owns 32 columns of S in its accumulators, where they stay in fp32 from chunk to chunk, and
+// computes those columns of O.  The products are transposed (P^T = K Q^T, O^T = S^T Q^T + V^T P^T), so that S and P go from
 // accumulator to operand without leaving the lane: the k index of an MFMA may be permuted as long as both operands agree, and
-// the order used throughout is the one the accumulators hold.  P passes through LDS, since every wave needs all of it.
+// the order used is the one the accumulators hold.  P is small (32 x 32) and computed by every wave for itself: that costs 8 of
+// 34 to 42 MFMAs and saves a round trip through LDS and a barrier.  The rows of S (and the columns of O) are numbered with bits
+// 2 and 3 swapped (sigma below), which makes the eight values of a lane in a k-step neighbours in memory: rows of Q and K are
+// read, and O written, 16 bytes at a time; the transposing reads of K and V swap two of their pieces instead, at no cost.
+// Tiles go from global memory straight to LDS, one chunk ahead.
 //
 // Roundings to 16 bits: S and P where they are operands of the product that gives O, as the scores of any tiled attention are
 // (one rounding each, against the one of O itself).  The state is an fp32 result, and it is carried over the whole sequence, so
-// there lam^(n-1-j) v_j is split into three bf16 parts, which hold its 24 bits.  fp16 tensors have three more bits than bf16
-// and a range that neither S nor P fits, so their operands are split into bf16 parts as well: two each for q, k, v (exact), S
-// and P, and products of the small parts are left out.
+// there lam^(n-1-j) v_j is split into three bf16 parts, which hold its 24 bits (two parts, 16 bits, where a segment's running
+// state only feeds O).  fp16 tensors have three more bits than bf16 and a range that neither S nor P fits, so their operands are
+// split into bf16 parts as well: two each for q, k, v (exact), S and P, and products of the small parts are left out.
 //
 // A few heads do not fill the chip.  The tokens are then cut into segments: one launch sums up each segment's own state, one
 // turns them into the states before each segment (elementwise, in order), and the kernel above runs all segments at once.
@@ -34,12 +38,12 @@ namespace linattn {
 using sdpa::lds_s16x4;
 using sdpa::s16x4;
 using sdpa::s16x8;
-using sdpa::static_for;
+using sdpa::f32x16;
+using sdpa::mma;
 using sdpa::swz_v;
 using sdpa::Vec8;
 
-constexpr int C = 64;         // tokens per chunk
-constexpr int P_ROW = 160;    // bytes per query row of P in LDS: 64 keys and a pad that spreads eight rows over the banks
+constexpr int C = 32;  // tokens per chunk
 constexpr float kLog2e = 1.44269504088896340736f;
 
 struct Operand {
@@ -71,8 +75,8 @@ struct Params {
   int n_seg, seg_chunks;
 };
 
-__device__ __forceinline__ f32x4 mma16(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x4 mma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// Row of an accumulator tile (or lane of an operand) -> row of S, column of V: bits 2 and 3 change places.
+__device__ __forceinline__ constexpr int sigma(int x) { return (x & 0x13) | ((x & 4) << 1) | ((x & 8) >> 1); }
 
 // A value in N bf16 parts, largest first.
 template <int N>
@@ -97,7 +101,7 @@ __device__ __forceinline__ Parts<N> split(const float (&x)[8]) {
   return p;
 }
 
-// An operand of the products that give O: one bf16 part for bf16 tensors, two for fp16.
+// Parts of an element of the tensors: bf16 is one, fp16 is two.
 template <typename T>
 constexpr int kParts = std::is_same_v<T, f16_t> ? 2 : 1;
 
@@ -115,41 +119,35 @@ __device__ __forceinline__ Parts<kParts<T>> as_parts(typename Vec8<T>::type x) {
 
 // Sum of the products of two split operands; parts i and j meet while i + j < max(NA, NB).
 template <int NA, int NB>
-__device__ __forceinline__ f32x4 mma_parts(const Parts<NA>& a, const Parts<NB>& b, f32x4 c) {
+__device__ __forceinline__ f32x16 mma_parts(const Parts<NA>& a, const Parts<NB>& b, f32x16 c) {
   constexpr int N = NA > NB ? NA : NB;
 #pragma unroll
   for (int i = NA - 1; i >= 0; --i)
 #pragma unroll
     for (int j = NB - 1; j >= 0; --j)
-      if (i + j < N) c = mma16(a.v[i], b.v[j], c);
+      if (i + j < N) c = mma(a.v[i], b.v[j], c);
   return c;
 }
 
-__device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-
+// A chunk's rows of one operand in LDS: [32][D], 16-byte pieces swizzled for both kinds of reads.
 template <typename T, int D>
 struct Tile {
   static constexpr int RB = D * 2;
   static constexpr int BYTES = C * RB;
   typedef typename Vec8<T>::type V8;
-  typedef T T4 __attribute__((ext_vector_type(4)));
 
-  // row `row`, columns 32 kk + 8 q4 .. +7
-  __device__ static __forceinline__ V8 row_frag(const char* tile, int row, int kk, int q4) {
-    return *reinterpret_cast<const V8*>(tile + row * RB + (((4 * kk + q4) ^ swz_v<D>(row)) << 4));
+  // row `row`, columns 16 t + 8 h .. +7
+  __device__ static __forceinline__ V8 row_frag(const char* tile, int row, int t, int h) {
+    return *reinterpret_cast<const V8*>(tile + row * RB + (((2 * t + h) ^ swz_v<D>(row)) << 4));
   }
-  // row `row`, columns 32 t + 4 q4 .. +3 and 32 t + 16 + 4 q4 .. +3
-  __device__ static __forceinline__ V8 row_frag_perm(const char* tile, int row, int t, int q4) {
-    const int sub = (q4 & 1) << 3, ch = 4 * t + (q4 >> 1);
-    const T4 lo = *reinterpret_cast<const T4*>(tile + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub);
-    const T4 hi = *reinterpret_cast<const T4*>(tile + row * RB + (((ch + 2) ^ swz_v<D>(row)) << 4) + sub);
-    return V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-  }
-  // column 16 ct + a16, rows 32 t + 4 q4 .. +3 and 32 t + 16 + 4 q4 .. +3 (two transposing reads)
-  __device__ static __forceinline__ V8 col_frag(const char* tile, int ct, int t, int q4, int a16) {
-    const int row = 32 * t + 4 * q4 + (a16 >> 2), ch = 2 * ct + ((a16 & 3) >> 1), sub = (a16 & 1) << 3;
+  // column 32 ct + sigma(lane % 32), rows 16 t + 4 h .. +3 and 16 t + 8 + 4 h .. +3: two transposing reads, in which sixteen lanes
+  // address four rows of four 8-byte pieces and lane i of them receives column i; the middle pieces are swapped
+  __device__ static __forceinline__ V8 col_frag(const char* tile, int ct, int t, int lane) {
+    const int h = lane >> 5, a16 = lane & 15, b16 = (lane >> 4) & 1;
+    const int piece = ((a16 & 1) << 1) | ((a16 >> 1) & 1);
+    const int row = 16 * t + 4 * h + (a16 >> 2), ch = 4 * ct + 2 * b16 + (piece >> 1), sub = (piece & 1) << 3;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (row + 16) * RB + ((ch ^ swz_v<D>(row + 16)) << 4) + sub));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (row + 8) * RB + ((ch ^ swz_v<D>(row + 8)) << 4) + sub));
     const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(V8, both);
   }
@@ -168,109 +166,146 @@ __device__ __forceinline__ float head_log2(const Params& p, int h) {
 }
 __device__ __forceinline__ float decay(float g2, int n) { return __builtin_amdgcn_exp2f(g2 * (float)n); }
 
-// The rows of one operand's chunk on their way from global memory to LDS.
+// An LDS address in a scalar register (the compiler would put a known constant, or one that it cannot tell to be uniform, into
+// a vector register).
+__device__ __forceinline__ uint32_t lds_address(const char* at) {
+  uint32_t x = (uint32_t)(uintptr_t)(sdpa::lvoid*)const_cast<char*>(at);
+  asm volatile("" : "+v"(x));
+  return __builtin_amdgcn_readfirstlane(x);
+}
+
+// One operand's chunks on their way from global memory to LDS.
 template <typename T, int D>
 struct Mover {
-  static constexpr int NT = D * 4;            // threads: D/16 waves
-  static constexpr int N = C * D / 8 / NT;    // 16-byte pieces per thread
-  const char* base;
-  int64_t row_bytes;                          // signed: a reversed operand walks backwards
-  u32x4 piece[N];
+  static constexpr int NT = D * 2;             // threads: D/32 waves
+  static constexpr int RB = D * 2;
+  const char* first;                           // token 0 in the order of the recurrence
+  int64_t row_bytes;                           // signed: a reversed operand walks backwards
+  uint32_t off[2];                             // this lane's part of the tile, from its lowest address
+  int64_t low;                                 // from the address of a chunk's first token to its lowest
 
-  __device__ __forceinline__ void bind(const Operand& o, int b, int h, int len, int reverse) {
+  __device__ __forceinline__ void bind(const Operand& o, int b, int head, int len, int reverse, int tid) {
     const int64_t last = reverse ? (int64_t)(len - 1) * o.s[2] : 0;
-    base = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (h / o.group) * o.s[1] + last) * 2;
+    first = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (head / o.group) * o.s[1] + last) * 2;
     row_bytes = (reverse ? -o.s[2] : o.s[2]) * 2;
-  }
-  __device__ __forceinline__ void load(int t0, int end, int tid) {
+    low = reverse ? (C - 1) * row_bytes : 0;
+    const uint32_t pitch = (uint32_t)(o.s[2] * 2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int idx = i * NT + tid, row = idx / (D / 8), c = idx % (D / 8);
-      piece[i] = u32x4{0, 0, 0, 0};
-      if (t0 + row < end) piece[i] = *reinterpret_cast<const u32x4*>(base + (int64_t)(t0 + row) * row_bytes + c * 16);
+    for (int i = 0; i < 2; ++i) {
+      const int pos = place(tid, i), row = pos / RB, pc = (pos % RB) >> 4;
+      off[i] = (uint32_t)(reverse ? C - 1 - row : row) * pitch + (uint32_t)((pc ^ swz_v<D>(row)) << 4);
     }
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
+  // bytes [1024 (2 wave + i) + 16 lane, + 16) of a tile
+  __device__ static __forceinline__ int place(int tid, int i) { return (2 * (tid >> 6) + i) * 1024 + (tid & 63) * 16; }
+
+  // 32 whole tokens from t0 on, straight to LDS (waits by vmcnt)
+  __device__ __forceinline__ void load(int t0, const char* tile, int w) const {
+    const uint64_t base = (uint64_t)(uintptr_t)(first + (int64_t)t0 * row_bytes + low);  // the same for every lane
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int idx = i * NT + tid, row = idx / (D / 8), c = idx % (D / 8);
-      *reinterpret_cast<u32x4*>(tile + row * (D * 2) + ((c ^ swz_v<D>(row)) << 4)) = piece[i];
+    for (int i = 0; i < 2; ++i) load_to_lds16((const void*)(uintptr_t)((uint64_t)hi << 32 | lo), off[i], lds_address(tile + (2 * w + i) * 1024));
+  }
+  // n < 32 tokens, zeros behind them
+  __device__ __forceinline__ void load_tail(int t0, int n, char* tile, int tid) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int pos = place(tid, i), row = pos / RB, pc = (pos % RB) >> 4;
+      u32x4 x = {0, 0, 0, 0};
+      if (row < n) x = *reinterpret_cast<const u32x4*>(first + (int64_t)(t0 + row) * row_bytes + ((pc ^ swz_v<D>(row)) << 4));
+      *reinterpret_cast<u32x4*>(tile + pos) = x;
     }
   }
 };
 
-// S' = lam^n S + sum_j f_j k_j v_j^T on this wave's 16 columns; f[t][jj] belongs to the token of slot jj of k-step t.
-template <typename T, int D>
-__device__ __forceinline__ void update_state(f32x4 (&S)[D / 16], const char* k_tile, const typename Vec8<T>::type (&vf)[2], const float (&f)[2][8],
-                                             float lam_n, int q4, int a16) {
+// The chunk loaded last is whole for every wave, and nobody reads the stage that comes next any more.
+__device__ __forceinline__ void chunk_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// S' = lam^n S + sum_j f_j k_j v_j^T on this wave's 32 columns; f[t][jj] belongs to the token of slot jj of k-step t.
+template <typename T, int D, int SP>
+__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], const char* k_tile, const typename Vec8<T>::type (&vf)[2], const float (&f)[2][8],
+                                             float lam_n, int lane) {
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) S[dt] *= lam_n;
+  for (int dt = 0; dt < D / 32; ++dt) S[dt] *= lam_n;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     float x[8];
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj) x[jj] = (float)vf[t][jj] * f[t][jj];
-    const Parts<3> fv = split<3>(x);
+    const Parts<SP> fv = split<SP>(x);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) S[dt] = mma_parts(as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, q4, a16)), fv, S[dt]);
+    for (int dt = 0; dt < D / 32; ++dt) S[dt] = mma_parts(as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, lane)), fv, S[dt]);
   }
 }
 
-__device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n, int e, float s_state, int q4) {
+__device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n, int e, float s_state, int h) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int jj = 0; jj < 8; ++jj) {
-      const int left = n - 1 - (32 * t + 4 * q4 + (jj & 3) + (jj < 4 ? 0 : 16));
+      const int left = n - 1 - (16 * t + 4 * h + (jj & 3) + (jj < 4 ? 0 : 8));
       f[t][jj] = decay(g2, left < 0 ? 0 : left + e) * s_state;
     }
 }
 
+// Where register 4 g + r of accumulator tile dt of a lane lies in a state.
+__device__ __forceinline__ int state_row(int dt, int g, int h) { return 32 * dt + 16 * (g >> 1) + 8 * h + 4 * (g & 1); }
+__device__ __forceinline__ int state_col(int w, int lane) { return 32 * w + sigma(lane & 31); }
+
 // Each segment's own state (from zero), in accumulator order.
 template <typename T, int D>
-__global__ __launch_bounds__(D * 4) void segment_states_kernel(const Params p) {
-  __shared__ __attribute__((aligned(1024))) char smem[2 * Tile<T, D>::BYTES];
-  char* k_s = smem;
-  char* v_s = smem + Tile<T, D>::BYTES;
+__global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void segment_states_kernel(const Params p) {
+  typedef Tile<T, D> TL;
+  __shared__ __attribute__((aligned(1024))) char smem[4 * TL::BYTES];  // two stages of K, V
   const Problem& pr = p.pr[blockIdx.y];
-  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, a16 = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
-  const int b = bh / p.H, h = bh % p.H;
-  const int len = length_of(p, b);
+  const int b = bh / p.H, head = bh % p.H;
+  const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C;
   const int t_end = t_beg + p.seg_chunks * C < len ? t_beg + p.seg_chunks * C : len;
   if (t_beg >= t_end) return;
-  const float g2 = head_log2(p, h);
-  f32x4 S[D / 16];
+  const float g2 = head_log2(p, head);
+  f32x16 S[D / 32];
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) S[dt][i] = 0.f;
   Mover<T, D> km, vm;
-  km.bind(pr.k, b, h, len, pr.reverse);
-  vm.bind(pr.v, b, h, len, pr.reverse);
+  km.bind(pr.k, b, head, len, pr.reverse, tid);
+  vm.bind(pr.v, b, head, len, pr.reverse, tid);
   float f[2][8];
-  token_factors(f, g2, C, pr.e, pr.s_state, q4);
-  km.load(t_beg, t_end, tid);
-  vm.load(t_beg, t_end, tid);
-  for (int t0 = t_beg; t0 < t_end; t0 += C) {
-    const int n = t_end - t0 < C ? t_end - t0 : C;
-    if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, q4);
-    lds_barrier();
-    km.store(k_s, tid);
-    vm.store(v_s, tid);
-    lds_barrier();
-    if (t0 + C < t_end) {
-      km.load(t0 + C, t_end, tid);
-      vm.load(t0 + C, t_end, tid);
+  token_factors(f, g2, C, pr.e, pr.s_state, h);
+  auto issue = [&](int t0, int stage) {
+    char* to = smem + stage * 2 * TL::BYTES;
+    if (t_end - t0 >= C) {
+      km.load(t0, to, w);
+      vm.load(t0, to + TL::BYTES, w);
+    } else {
+      km.load_tail(t0, t_end - t0, to, tid);
+      vm.load_tail(t0, t_end - t0, to + TL::BYTES, tid);
     }
-    typename Vec8<T>::type vf[2];
+  };
+  issue(t_beg, 0);
+  int stage = 0;
+  for (int t0 = t_beg; t0 < t_end; t0 += C, stage ^= 1) {
+    const int n = t_end - t0 < C ? t_end - t0 : C;
+    if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, h);
+    chunk_barrier();
+    if (t0 + C < t_end) issue(t0 + C, stage ^ 1);
+    const char* k_s = smem + stage * 2 * TL::BYTES;
+    typename TL::V8 vf[2];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) vf[t] = Tile<T, D>::col_frag(v_s, w, t, q4, a16);
-    update_state<T, D>(S, k_s, vf, f, decay(g2, n), q4, a16);
+    for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(k_s + TL::BYTES, w, t, lane);
+    update_state<T, D, 3>(S, k_s, vf, f, decay(g2, n), lane);
   }
   float* to = pr.seg_states + (int64_t)blockIdx.x * (D * D);
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(to + ((w * (D / 16) + dt) * 64 + lane) * 4) = S[dt];
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      *reinterpret_cast<f32x4*>(to + (((w * (D / 32) + dt) * 4 + g) * 64 + lane) * 4) = f32x4{S[dt][4 * g], S[dt][4 * g + 1], S[dt][4 * g + 2], S[dt][4 * g + 3]};
 }
 
 // Segment states in order: what segment m added becomes the state before segment m.  One thread per four elements.
@@ -280,11 +315,11 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
   constexpr int PER = D * D / 1024;  // blocks per head
   const int bh = blockIdx.x / PER;
   const int at = (blockIdx.x % PER) * 1024 + threadIdx.x * 4;
-  const int b = bh / p.H, h = bh % p.H;
-  const int lane = (at >> 2) & 63, dt = (at >> 8) % (D / 16), w = (at >> 8) / (D / 16);
-  const int dk = 16 * dt + 4 * (lane >> 4), dv = 16 * w + (lane & 15);
+  const int b = bh / p.H, head = bh % p.H;
+  const int lane = (at >> 2) & 63, g = (at >> 8) & 3, dt = (at >> 10) % (D / 32), w = (at >> 10) / (D / 32);
+  const int dk = state_row(dt, g, lane >> 5), dv = state_col(w, lane);
   const int len = length_of(p, b);
-  const float g2 = head_log2(p, h);
+  const float g2 = head_log2(p, head);
   f32x4 S = {0.f, 0.f, 0.f, 0.f};
   if (pr.state0) {
     const float* s0 = pr.state0 + (int64_t)bh * (D * D);
@@ -309,35 +344,31 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
   }
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(D * 4) void linear_attn_kernel(const Params p) {
+// SP: parts of the running state's update (three where the state is a result, two where it only feeds O).
+template <typename T, int D, int SP>
+__global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_attn_kernel(const Params p) {
   typedef typename Vec8<T>::type V8;
   typedef Tile<T, D> TL;
-  constexpr int NW = D / 16;                       // waves
-  constexpr int NP = (10 + NW - 1) / NW;           // tiles of P per wave (10 of the 4 x 4 lie on or below the diagonal)
-  constexpr int PP = kParts<T>;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];
-  char* q_s = smem;
-  char* k_s = smem + TL::BYTES;
-  char* v_s = smem + 2 * TL::BYTES;
-  char* p_s = smem + 3 * TL::BYTES;                // [PP][64 queries][P_ROW bytes]
+  constexpr int OP = kParts<T>;  // parts of S and P as operands of O
+  constexpr int STAGE = 3 * TL::BYTES;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of Q, K, V
   const Problem& pr = p.pr[blockIdx.y];
-  const int tid = threadIdx.x, lane = tid & 63, q4 = lane >> 4, a16 = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
-  const int b = bh / p.H, h = bh % p.H;
-  const int len = length_of(p, b);
+  const int b = bh / p.H, head = bh % p.H;
+  const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C;
   const int s_end = t_beg + p.seg_chunks * C < p.S ? t_beg + p.seg_chunks * C : p.S;
   const int t_end = s_end < len ? s_end : len;
-  const float g2 = head_log2(p, h);
+  const float g2 = head_log2(p, head);
+  const int64_t out0 = b * pr.os[0] + head * pr.os[1];
 
   // rows behind the sequence: zeros
   {
     const int from = t_beg > len ? t_beg : len;
-    const int64_t row0 = b * pr.os[0] + h * pr.os[1];
-    for (int idx = tid; idx < (s_end - from) * (D / 8); idx += D * 4) {
-      const int64_t at = row0 + (int64_t)(from + idx / (D / 8)) * pr.os[2] + (idx % (D / 8)) * 8;
+    for (int idx = tid; idx < (s_end - from) * (D / 8); idx += D * 2) {
+      const int64_t at = out0 + (int64_t)(from + idx / (D / 8)) * pr.os[2] + (idx % (D / 8)) * 8;
       const u32x4 zero = {0, 0, 0, 0};
       if (pr.out_f32) {
         u32x4* o = reinterpret_cast<u32x4*>(reinterpret_cast<float*>(pr.out) + at);
@@ -350,166 +381,136 @@ __global__ __launch_bounds__(D * 4) void linear_attn_kernel(const Params p) {
   }
 
   // the state before the segment
-  f32x4 S[D / 16];
+  f32x16 S[D / 32];
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt) S[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) S[dt][i] = 0.f;
   if (p.n_seg > 1) {
     if (t_beg >= t_end) return;
     const float* from = pr.seg_states + (int64_t)blockIdx.x * (D * D);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) S[dt] = *reinterpret_cast<const f32x4*>(from + ((w * (D / 16) + dt) * 64 + lane) * 4);
+    for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 x = *reinterpret_cast<const f32x4*>(from + (((w * (D / 32) + dt) * 4 + g) * 64 + lane) * 4);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[dt][4 * g + r] = x[r];
+      }
   } else if (pr.state0) {
     const float* s0 = pr.state0 + (int64_t)bh * (D * D);
+    const int dv = state_col(w, lane);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int dk = 16 * dt + 4 * q4 + r, dv = 16 * w + a16;
-        S[dt][r] = pr.state0_t ? s0[dv * D + dk] : s0[dk * D + dv];
+      for (int i = 0; i < 16; ++i) {
+        const int dk = state_row(dt, i >> 2, h) + (i & 3);
+        S[dt][i] = pr.state0_t ? s0[dv * D + dk] : s0[dk * D + dv];
       }
   }
   const bool keep_state = p.n_seg == 1 && pr.state_out;
 
   if (t_beg < t_end) {
     Mover<T, D> qm, km, vm;
-    qm.bind(pr.q, b, h, len, pr.reverse);
-    km.bind(pr.k, b, h, len, pr.reverse);
-    vm.bind(pr.v, b, h, len, pr.reverse);
-    qm.load(t_beg, t_end, tid);
-    km.load(t_beg, t_end, tid);
-    vm.load(t_beg, t_end, tid);
+    qm.bind(pr.q, b, head, len, pr.reverse, tid);
+    km.bind(pr.k, b, head, len, pr.reverse, tid);
+    vm.bind(pr.v, b, head, len, pr.reverse, tid);
+    auto issue = [&](int t0, int stage) {
+      char* to = smem + stage * STAGE;
+      if (t_end - t0 >= C) {
+        qm.load(t0, to, w);
+        km.load(t0, to + TL::BYTES, w);
+        vm.load(t0, to + 2 * TL::BYTES, w);
+      } else {
+        qm.load_tail(t0, t_end - t0, to, tid);
+        km.load_tail(t0, t_end - t0, to + TL::BYTES, tid);
+        vm.load_tail(t0, t_end - t0, to + 2 * TL::BYTES, tid);
+      }
+    };
+    issue(t_beg, 0);
 
     // factors that do not change from chunk to chunk
     float f[2][8];
-    token_factors(f, g2, C, pr.e, pr.s_state, q4);
-    float row_f[4];
+    token_factors(f, g2, C, pr.e, pr.s_state, h);
+    const float row_f = decay(g2, l32 + 1 - pr.e) * pr.s_inter;
+    float p_f[16];  // of P^T: lane = query, register 4 g + r = key 8 g + 4 h + r
 #pragma unroll
-    for (int qt = 0; qt < 4; ++qt) row_f[qt] = decay(g2, 16 * qt + a16 + 1 - pr.e) * pr.s_inter;
-    float p_f[NP][4];
-    int p_kt[NP], p_qt[NP];
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int id = w + NW * i;
-      p_qt[i] = id >= 6 ? 3 : (id >= 3 ? 2 : (id >= 1 ? 1 : 0));
-      p_kt[i] = id - p_qt[i] * (p_qt[i] + 1) / 2;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int d = 16 * (p_qt[i] - p_kt[i]) + a16 - 4 * q4 - r;
-        p_f[i][r] = d < 0 ? 0.f : decay(g2, d) * pr.s_intra;
-      }
-    }
-    // the two tiles of P above the diagonal that the 32-key steps read: always zero
-    for (int idx = tid; idx < PP * 2 * 16 * 2; idx += D * 4) {
-      const int half = idx & 1, row = (idx >> 1) & 15, which = (idx >> 5) & 1, part = idx >> 6;
-      *reinterpret_cast<u32x4*>(p_s + part * C * P_ROW + (32 * which + row) * P_ROW + (32 * which + 16) * 2 + half * 16) = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < 16; ++i) {
+      const int d = l32 - (8 * (i >> 2) + 4 * h + (i & 3));
+      p_f[i] = d < 0 ? 0.f : decay(g2, d) * pr.s_intra;
     }
 
-    for (int t0 = t_beg; t0 < t_end; t0 += C) {
+    int stage = 0;
+    for (int t0 = t_beg; t0 < t_end; t0 += C, stage ^= 1) {
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      lds_barrier();  // every wave is done with the previous chunk's tiles
-      qm.store(q_s, tid);
-      km.store(k_s, tid);
-      vm.store(v_s, tid);
-      lds_barrier();
-      if (t0 + C < t_end) {
-        qm.load(t0 + C, t_end, tid);
-        km.load(t0 + C, t_end, tid);
-        vm.load(t0 + C, t_end, tid);
-      }
+      chunk_barrier();
+      if (t0 + C < t_end) issue(t0 + C, stage ^ 1);
+      const char* q_s = smem + stage * STAGE;
+      const char* k_s = q_s + TL::BYTES;
+      const char* v_s = q_s + 2 * TL::BYTES;
 
-      // P^T = K Q^T, decayed
+      // P^T = K Q^T and O^T = S^T Q^T from the same rows of Q; each query of O scaled by its decay
+      f32x16 P, O;
 #pragma unroll
-      for (int i = 0; i < NP; ++i) {
-        if (w + NW * i < 10) {
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < 16; ++i) P[i] = O[i] = 0.f;
 #pragma unroll
-          for (int kk = 0; kk < D / 32; ++kk)
-            acc = mma16(TL::row_frag(k_s, 16 * p_kt[i] + a16, kk, q4), TL::row_frag(q_s, 16 * p_qt[i] + a16, kk, q4), acc);
-          char* to = p_s + (16 * p_qt[i] + a16) * P_ROW + (16 * p_kt[i] + 4 * q4) * 2;
-          float x[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) x[r] = 16 * (p_qt[i] - p_kt[i]) + a16 - 4 * q4 - r >= 0 ? acc[r] * p_f[i][r] : 0.f;
-#pragma unroll
-          for (int part = 0; part < PP; ++part) {
-            bf16x4 y;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              y[r] = (bf16_t)x[r];
-              x[r] -= (float)y[r];
-            }
-            *reinterpret_cast<bf16x4*>(to + part * C * P_ROW) = y;
-          }
-        }
-      }
-
-      // O^T = S^T Q^T, each query scaled by its decay
-      f32x4 O[4];
-#pragma unroll
-      for (int qt = 0; qt < 4; ++qt) O[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
+      for (int t = 0; t < D / 16; ++t) {
+        const V8 qf = TL::row_frag(q_s, l32, t, h);
+        P = mma(TL::row_frag(k_s, l32, t, h), qf, P);
         float x[8];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) x[r] = S[2 * t][r], x[4 + r] = S[2 * t + 1][r];
-        const Parts<PP> sp = split<PP>(x);
-#pragma unroll
-        for (int qt = 0; qt < 4; ++qt) O[qt] = mma_parts(sp, as_parts<T>(TL::row_frag_perm(q_s, 16 * qt + a16, t, q4)), O[qt]);
+        for (int i = 0; i < 8; ++i) x[i] = S[t >> 1][8 * (t & 1) + i];
+        O = mma_parts(split<OP>(x), as_parts<T>(qf), O);
       }
-#pragma unroll
-      for (int qt = 0; qt < 4; ++qt) O[qt] *= row_f[qt];
+      O *= row_f;
       V8 vf[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(v_s, w, t, q4, a16);
-      lds_barrier();  // P is whole
+      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(v_s, w, t, lane);
 
       // O^T += V^T P^T
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const Parts<PP> vp = as_parts<T>(vf[t]);
+        float x[8];
 #pragma unroll
-        for (int qt = 2 * t; qt < 4; ++qt) {
-          Parts<PP> pp;
-#pragma unroll
-          for (int part = 0; part < PP; ++part) {
-            const char* row = p_s + part * C * P_ROW + (16 * qt + a16) * P_ROW + (32 * t + 4 * q4) * 2;
-            const bf16x4 lo = *reinterpret_cast<const bf16x4*>(row), hi = *reinterpret_cast<const bf16x4*>(row + 32);
-            pp.v[part] = bf16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-          }
-          O[qt] = mma_parts(vp, pp, O[qt]);
-        }
+        for (int i = 0; i < 8; ++i) x[i] = P[8 * t + i] * p_f[8 * t + i];
+        O = mma_parts(as_parts<T>(vf[t]), split<OP>(x), O);
       }
 
-      // lane: query 16 qt + a16, columns 16 w + 4 q4 .. +3
+      // lane: query l32, columns 32 w + 16 t + 8 h .. +7 in registers 8 t .. 8 t + 7
+      if (l32 < n) {
+        const int64_t token = pr.reverse ? (int64_t)len - 1 - (t0 + l32) : (int64_t)t0 + l32;
+        const int64_t at = out0 + token * pr.os[2] + 32 * w + 8 * h;
+        if (pr.out_f32) {
+          float* o = reinterpret_cast<float*>(pr.out) + at;
 #pragma unroll
-      for (int qt = 0; qt < 4; ++qt) {
-        const int row = 16 * qt + a16;
-        if (row < n) {
-          const int64_t token = pr.reverse ? (int64_t)len - 1 - (t0 + row) : (int64_t)t0 + row;
-          const int64_t at = b * pr.os[0] + h * pr.os[1] + token * pr.os[2] + 16 * w + 4 * q4;
-          if (pr.out_f32) {
-            *reinterpret_cast<f32x4*>(reinterpret_cast<float*>(pr.out) + at) = O[qt];
-          } else {
-            typename TL::T4 y;
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(o + 16 * (g >> 1) + 4 * (g & 1)) = f32x4{O[4 * g], O[4 * g + 1], O[4 * g + 2], O[4 * g + 3]};
+        } else {
+          T* o = reinterpret_cast<T*>(pr.out) + at;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = (T)O[qt][r];
-            *reinterpret_cast<typename TL::T4*>(reinterpret_cast<T*>(pr.out) + at) = y;
+          for (int t = 0; t < 2; ++t) {
+            V8 y;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = (T)O[8 * t + i];
+            *reinterpret_cast<V8*>(o + 16 * t) = y;
           }
         }
       }
 
       if (t0 + C < t_end || keep_state) {
-        if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, q4);
-        update_state<T, D>(S, k_s, vf, f, decay(g2, n), q4, a16);
+        if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, h);
+        update_state<T, D, SP>(S, k_s, vf, f, decay(g2, n), lane);
       }
     }
   }
 
   if (keep_state) {
     float* so = pr.state_out + (int64_t)bh * (D * D);
+    const int dv = state_col(w, lane);
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt)
+    for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) so[(16 * dt + 4 * q4 + r) * D + 16 * w + a16] = S[dt][r];
+      for (int i = 0; i < 16; ++i) so[(state_row(dt, i >> 2, h) + (i & 3)) * D + dv] = S[dt][i];
   }
 }
 
@@ -599,13 +600,15 @@ __global__ __launch_bounds__(256) void linear_attn_step_kernel(const StepParams 
 }
 
 // ------------------------------------------------------------------ host side
+constexpr int64_t kMaxPitch = 1 << 26;  // elements between tokens: 32 rows stay inside 32-bit offsets
+
 int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
 
-// How many segments the tokens of a head are cut into: enough workgroups to fill the chip twice over, at least two chunks each.
+// How many segments the tokens of a head are cut into: enough workgroups to fill the chip twice over, at least four chunks each.
 void segments(int64_t heads, int64_t S, int& n_seg, int& seg_chunks) {
   const int64_t chunks = chunks_of(S);
   int64_t n = (512 + heads - 1) / heads;
-  if (n > chunks / 2) n = chunks / 2;
+  if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   seg_chunks = (int)((chunks + n - 1) / n);
   n_seg = (int)((chunks + seg_chunks - 1) / seg_chunks);
@@ -627,7 +630,7 @@ int fill(int64_t (&to)[3], const int64_t* from) {
     if (from[i] % 8) return XG_ERR_BAD_ALIGN;
     to[i] = from[i];
   }
-  return XG_OK;
+  return from[2] < kMaxPitch ? XG_OK : XG_ERR_TOO_LARGE;
 }
 
 int fill(Operand& o, const void* p, const int64_t* s, int group) {
@@ -640,15 +643,14 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
-  constexpr int SMEM = 3 * Tile<T, D>::BYTES + kParts<T> * C * P_ROW;
-  auto kernel = linear_attn_kernel<T, D>;
-  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), SMEM)) return rc;
-  const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems);
+  const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), block(D * 2);
   if (p.n_seg > 1) {
-    hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, dim3(D * 4), 0, st, p);
+    hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, block, 0, st, p);
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), grid, block, 0, st, p);
+  } else {
+    hipLaunchKernelGGL((linear_attn_kernel<T, D, 3>), grid, block, 0, st, p);
   }
-  hipLaunchKernelGGL(kernel, grid, dim3(D * 4), SMEM, st, p);
   return status_from_hip(hipGetLastError());
 }
 
