@@ -73,6 +73,7 @@ struct Params {
   int len64;
   int B, H, S;
   int n_seg, seg_chunks;
+  int stages;               // chunks in LDS
 };
 
 // Row of an accumulator tile (or lane of an operand) -> row of S, column of V: bits 2 and 3 change places.
@@ -218,26 +219,40 @@ struct Mover {
   }
 };
 
-// The chunk loaded last is whole for every wave, and nobody reads the stage that comes next any more.
-__device__ __forceinline__ void chunk_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// This chunk is whole for every wave, and nobody reads the stage that is filled next any more.  LATER: vector memory operations
+// of this wave that were issued after the chunk's loads and may still be in flight (they end in order).
+template <int LATER>
+__device__ __forceinline__ void chunk_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+}
 
-// S' = lam^n S + sum_j f_j k_j v_j^T on this wave's 32 columns; f[t][jj] belongs to the token of slot jj of k-step t.
-template <typename T, int D, int SP>
-__device__ __forceinline__ void update_state(f32x16 (&S)[D / 32], const char* k_tile, const typename Vec8<T>::type (&vf)[2], const float (&f)[2][8],
-                                             float lam_n, int lane) {
-#pragma unroll
-  for (int dt = 0; dt < D / 32; ++dt) S[dt] *= lam_n;
+// S += sum_j x_j k_j on this wave's 32 columns, x[t][jj] the weighed value of the token in slot jj of k-step t.
+// Three bf16 parts of x where the state is a result (`whole`), two where it only feeds O.
+template <typename T, int D>
+__device__ __forceinline__ void add_to_state(f32x16 (&S)[D / 32], const char* k_tile, float (&x)[2][8], bool whole, int lane) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    float x[8];
+    const Parts<2> xv = split<2>(x[t]);
+    Parts<kParts<T>> kf[D / 32];
 #pragma unroll
-    for (int jj = 0; jj < 8; ++jj) x[jj] = (float)vf[t][jj] * f[t][jj];
-    const Parts<SP> fv = split<SP>(x);
+    for (int dt = 0; dt < D / 32; ++dt) {
+      kf[dt] = as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, lane));
+      S[dt] = mma_parts(kf[dt], xv, S[dt]);
+    }
+    if (whole) {
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt) S[dt] = mma_parts(as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, lane)), fv, S[dt]);
+      for (int jj = 0; jj < 8; ++jj) x[t][jj] = (x[t][jj] - (float)xv.v[0][jj]) - (float)xv.v[1][jj];
+      const Parts<1> rest = split<1>(x[t]);
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt) {
+        S[dt] = mma(kf[dt].v[0], rest.v[0], S[dt]);
+        if constexpr (kParts<T> == 2) S[dt] = mma(kf[dt].v[1], xv.v[1], S[dt]);
+      }
+    }
   }
 }
 
+// lam^(n-1-j+e) for the tokens j of this lane's slots in a chunk of n.
 __device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n, int e, float s_state, int h) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -252,21 +267,29 @@ __device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n,
 __device__ __forceinline__ int state_row(int dt, int g, int h) { return 32 * dt + 16 * (g >> 1) + 8 * h + 4 * (g & 1); }
 __device__ __forceinline__ int state_col(int w, int lane) { return 32 * w + sigma(lane & 31); }
 
-// Each segment's own state (from zero), in accumulator order.
+// Each segment's own state (from zero), in accumulator order; that of the last one is not needed, so segments are whole here.
+// Every token is weighed for the end of the segment at once.  Chunks whose weights are all zero in fp32 (lam^n below 2^-150) add
+// nothing and are not read.
 template <typename T, int D>
 __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void segment_states_kernel(const Params p) {
   typedef Tile<T, D> TL;
-  __shared__ __attribute__((aligned(1024))) char smem[4 * TL::BYTES];  // two stages of K, V
+  constexpr int STAGE = 2 * TL::BYTES;
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of K, V
   const Problem& pr = p.pr[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
+  const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = blockIdx.x % heads;  // neighbours in a token run side by side
   const int b = bh / p.H, head = bh % p.H;
   const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
-  const int t_beg = seg * p.seg_chunks * C;
-  const int t_end = t_beg + p.seg_chunks * C < len ? t_beg + p.seg_chunks * C : len;
-  if (t_beg >= t_end) return;
+  const int t_beg = seg * p.seg_chunks * C, t_end = t_beg + p.seg_chunks * C;
+  if (t_end >= len) return;  // nothing comes after
   const float g2 = head_log2(p, head);
+  int t0 = t_beg;
+  if (g2 < 0.f) {
+    const float live = 150.f / -g2;
+    if (live < (float)(t_end - t_beg)) t0 = max(t_beg, t_end - ((int)live / C + 1) * C);
+  }
+  t0 = __builtin_amdgcn_readfirstlane(t0);
   f32x16 S[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -277,30 +300,26 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   vm.bind(pr.v, b, head, len, pr.reverse, tid);
   float f[2][8];
   token_factors(f, g2, C, pr.e, pr.s_state, h);
-  auto issue = [&](int t0, int stage) {
-    char* to = smem + stage * 2 * TL::BYTES;
-    if (t_end - t0 >= C) {
-      km.load(t0, to, w);
-      vm.load(t0, to + TL::BYTES, w);
-    } else {
-      km.load_tail(t0, t_end - t0, to, tid);
-      vm.load_tail(t0, t_end - t0, to + TL::BYTES, tid);
+  km.load(t0, smem, w);
+  vm.load(t0, smem + TL::BYTES, w);
+  for (int stage = 0; t0 < t_end; t0 += C, stage ^= 1) {
+    chunk_barrier<0>();
+    if (t0 + C < t_end) {
+      km.load(t0 + C, smem + (stage ^ 1) * STAGE, w);
+      vm.load(t0 + C, smem + (stage ^ 1) * STAGE + TL::BYTES, w);
     }
-  };
-  issue(t_beg, 0);
-  int stage = 0;
-  for (int t0 = t_beg; t0 < t_end; t0 += C, stage ^= 1) {
-    const int n = t_end - t0 < C ? t_end - t0 : C;
-    if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, h);
-    chunk_barrier();
-    if (t0 + C < t_end) issue(t0 + C, stage ^ 1);
-    const char* k_s = smem + stage * 2 * TL::BYTES;
-    typename TL::V8 vf[2];
+    const char* k_s = smem + stage * STAGE;
+    const float rest = decay(g2, t_end - t0 - C);
+    float x[2][8];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(k_s + TL::BYTES, w, t, lane);
-    update_state<T, D, 3>(S, k_s, vf, f, decay(g2, n), lane);
+    for (int t = 0; t < 2; ++t) {
+      const typename TL::V8 vf = TL::col_frag(k_s + TL::BYTES, w, t, lane);
+#pragma unroll
+      for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[jj] * (f[t][jj] * rest);
+    }
+    add_to_state<T, D>(S, k_s, x, true, lane);
   }
-  float* to = pr.seg_states + (int64_t)blockIdx.x * (D * D);
+  float* to = pr.seg_states + ((int64_t)bh * p.n_seg + seg) * (D * D);
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -328,34 +347,32 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
   }
   float* ws = pr.seg_states + (int64_t)bh * p.n_seg * (D * D) + at;
   const int seg_len = p.seg_chunks * C;
-  for (int m = 0; m < p.n_seg; ++m) {
-    const int left = len - m * seg_len;
-    const int n = left < 0 ? 0 : (left < seg_len ? left : seg_len);
+  for (int m = 0; m * seg_len < len; ++m) {
     f32x4* cell = reinterpret_cast<f32x4*>(ws + (int64_t)m * (D * D));
-    if (n == 0) break;  // no segment from here on has tokens
-    const f32x4 own = *cell;
+    const bool last = (m + 1) * seg_len >= len;
+    f32x4 own = {0.f, 0.f, 0.f, 0.f};
+    if (!last) own = *cell;
     *cell = S;
-    S = S * decay(g2, n) + own;
+    S = S * decay(g2, seg_len) + own;
   }
-  if (pr.state_out) {
+  if (len == 0 && pr.state_out) {  // otherwise the last segment ends with it
     float* so = pr.state_out + (int64_t)bh * (D * D);
 #pragma unroll
     for (int r = 0; r < 4; ++r) so[(dk + r) * D + dv] = S[r];
   }
 }
 
-// SP: parts of the running state's update (three where the state is a result, two where it only feeds O).
-template <typename T, int D, int SP>
+template <typename T, int D>
 __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_attn_kernel(const Params p) {
   typedef typename Vec8<T>::type V8;
   typedef Tile<T, D> TL;
   constexpr int OP = kParts<T>;  // parts of S and P as operands of O
   constexpr int STAGE = 3 * TL::BYTES;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of Q, K, V
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // stages of Q, K, V
   const Problem& pr = p.pr[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int bh = blockIdx.x / p.n_seg, seg = blockIdx.x % p.n_seg;
+  const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = blockIdx.x % heads;  // neighbours in a token run side by side
   const int b = bh / p.H, head = bh % p.H;
   const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C;
@@ -388,7 +405,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     for (int i = 0; i < 16; ++i) S[dt][i] = 0.f;
   if (p.n_seg > 1) {
     if (t_beg >= t_end) return;
-    const float* from = pr.seg_states + (int64_t)blockIdx.x * (D * D);
+    const float* from = pr.seg_states + ((int64_t)bh * p.n_seg + seg) * (D * D);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
@@ -408,7 +425,10 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         S[dt][i] = pr.state0_t ? s0[dv * D + dk] : s0[dk * D + dv];
       }
   }
-  const bool keep_state = p.n_seg == 1 && pr.state_out;
+  // the loads above end here: left to the first use, the wait for them would stand inside the loop and hold up its prefetch
+#pragma unroll
+  for (int dt = 0; dt < D / 32; ++dt) asm volatile("" : "+v"(S[dt]));
+  const bool keep_state = pr.state_out && (p.n_seg == 1 || (t_beg < t_end && t_end == len));  // this segment ends with the last token
 
   if (t_beg < t_end) {
     Mover<T, D> qm, km, vm;
@@ -416,6 +436,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     km.bind(pr.k, b, head, len, pr.reverse, tid);
     vm.bind(pr.v, b, head, len, pr.reverse, tid);
     auto issue = [&](int t0, int stage) {
+      if (t0 >= t_end) return;
       char* to = smem + stage * STAGE;
       if (t_end - t0 >= C) {
         qm.load(t0, to, w);
@@ -427,7 +448,8 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         vm.load_tail(t0, t_end - t0, to + 2 * TL::BYTES, tid);
       }
     };
-    issue(t_beg, 0);
+    const int ahead = p.stages - 1;  // chunks in flight: one or two
+    for (int i = 0; i < ahead; ++i) issue(t_beg + i * C, i);
 
     // factors that do not change from chunk to chunk
     float f[2][8];
@@ -441,10 +463,15 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     }
 
     int stage = 0;
-    for (int t0 = t_beg; t0 < t_end; t0 += C, stage ^= 1) {
+    for (int t0 = t_beg; t0 < t_end; t0 += C, stage = stage == ahead ? 0 : stage + 1) {
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      chunk_barrier();
-      if (t0 + C < t_end) issue(t0 + C, stage ^ 1);
+      if (ahead == 1 || t0 + C >= t_end)
+        chunk_barrier<0>();
+      else if (t0 < t_beg + 2 * C)  // the next chunk's six loads have been issued since
+        chunk_barrier<6>();
+      else  // and the stores (two or more) of one chunk at least
+        chunk_barrier<8>();
+      issue(t0 + ahead * C, stage == 0 ? ahead : stage - 1);
       const char* q_s = smem + stage * STAGE;
       const char* k_s = q_s + TL::BYTES;
       const char* v_s = q_s + 2 * TL::BYTES;
@@ -499,7 +526,15 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
       if (t0 + C < t_end || keep_state) {
         if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, h);
-        update_state<T, D, SP>(S, k_s, vf, f, decay(g2, n), lane);
+        const float lam_n = decay(g2, n);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt) S[dt] *= lam_n;
+        float x[2][8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[t][jj] * f[t][jj];
+        add_to_state<T, D>(S, k_s, x, keep_state, lane);
       }
     }
   }
@@ -605,13 +640,20 @@ constexpr int64_t kMaxPitch = 1 << 26;  // elements between tokens: 32 rows stay
 int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
 
 // How many segments the tokens of a head are cut into: enough workgroups to fill the chip twice over, at least four chunks each.
-void segments(int64_t heads, int64_t S, int& n_seg, int& seg_chunks) {
-  const int64_t chunks = chunks_of(S);
-  int64_t n = (512 + heads - 1) / heads;
+void segments(int64_t heads, int64_t n_problems, int64_t S, int& n_seg, int& seg_chunks) {
+  const int64_t chunks = chunks_of(S), groups = heads * n_problems;
+  int64_t n = groups >= 256 ? 1 : (512 + groups - 1) / groups;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   seg_chunks = (int)((chunks + n - 1) / n);
   n_seg = (int)((chunks + seg_chunks - 1) / seg_chunks);
+}
+
+// Floats of the segment states of one problem.
+int64_t state_floats(int64_t heads, int64_t n_problems, int64_t S, int64_t D) {
+  int n_seg, seg_chunks;
+  segments(heads, n_problems, S, n_seg, seg_chunks);
+  return n_seg > 1 ? heads * n_seg * D * D : 0;
 }
 
 int check(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D, float scale, int dtype) {
@@ -643,14 +685,15 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
+  auto kernel = linear_attn_kernel<T, D>;
+  constexpr int STAGE = 3 * Tile<T, D>::BYTES;
+  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 3 * STAGE)) return rc;
   const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), block(D * 2);
   if (p.n_seg > 1) {
     hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, block, 0, st, p);
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
-    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), grid, block, 0, st, p);
-  } else {
-    hipLaunchKernelGGL((linear_attn_kernel<T, D, 3>), grid, block, 0, st, p);
   }
+  hipLaunchKernelGGL(kernel, grid, block, p.stages * STAGE, st, p);
   return status_from_hip(hipGetLastError());
 }
 
@@ -665,9 +708,7 @@ int launch_any(const Params& p, int n_problems, int64_t D, int dtype, hipStream_
 extern "C" int64_t xg_linear_attn_workspace_floats(int64_t B, int64_t H, int64_t S, int64_t D) {
   using namespace xg::linattn;
   if (check(B, H, H, S, D, 1.f, XG_BF16) != XG_OK || B == 0 || H == 0 || S == 0) return 0;
-  int n_seg, seg_chunks;
-  segments(B * H, S, n_seg, seg_chunks);
-  return n_seg > 1 ? B * H * n_seg * D * D : 0;
+  return state_floats(B * H, 1, S, D);
 }
 
 extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const float* log_decay, const float* state, const void* lengths,
@@ -694,7 +735,8 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
   p.B = (int)B;
   p.H = (int)H;
   p.S = (int)S;
-  segments(B * H, S, p.n_seg, p.seg_chunks);
+  segments(B * H, 1, S, p.n_seg, p.seg_chunks);
+  p.stages = p.n_seg > 1 ? 2 : 3;
   if (p.n_seg > 1) {
     if (!workspace) return XG_ERR_NULL_PTR;
     if (workspace_floats < B * H * p.n_seg * D * D) return XG_ERR_BAD_ARG;
@@ -712,7 +754,7 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
 extern "C" int64_t xg_linear_attn_bwd_workspace_floats(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D) {
   using namespace xg::linattn;
   if (check(B, H, Hkv, S, D, 1.f, XG_BF16) != XG_OK || B == 0 || H == 0 || S == 0) return 0;
-  return 3 * xg_linear_attn_workspace_floats(B, H, S, D) + (H != Hkv ? 2 * B * H * S * D : 0);
+  return 3 * state_floats(B * H, 3, S, D) + (H != Hkv ? 2 * B * H * S * D : 0);
 }
 
 extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, const float* log_decay, const float* state, const void* lengths,
@@ -743,13 +785,14 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   p.B = (int)B;
   p.H = (int)H;
   p.S = (int)S;
-  segments(B * H, S, p.n_seg, p.seg_chunks);
+  segments(B * H, 3, S, p.n_seg, p.seg_chunks);
+  p.stages = p.n_seg > 1 ? 2 : 3;
   const int64_t need = xg_linear_attn_bwd_workspace_floats(B, H, Hkv, S, D);
   if (need) {
     if (!workspace) return XG_ERR_NULL_PTR;
     if (workspace_floats < need) return XG_ERR_BAD_ARG;
   }
-  const int64_t seg_floats = p.n_seg > 1 ? B * H * p.n_seg * D * D : 0;
+  const int64_t seg_floats = state_floats(B * H, 3, S, D);
   float* partial = workspace + 3 * seg_floats;
   // dq = scale F(do, v, k), its state the transpose of the forward's
   Problem& a = p.pr[0];
