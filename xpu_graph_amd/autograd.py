@@ -283,59 +283,97 @@ def _rope_backward(ctx, gy):
     return gx, gcos, gsin
 
 
-def _refuse_table_grad(ctx, name, cos):
-    if ctx.needs_input_grad[cos] or ctx.needs_input_grad[cos + 1]:
-        raise NotImplementedError(f"xpu_ops::{name}: no gradient for the cos / sin tables")
+# The three ops below go through torch.autograd.Function at the Autograd dispatch key instead of register_autograd: the
+# bookkeeping of the latter (defaults, metadata and pytrees of every call) costs 15 to 30 us a call, more than their kernels take
+# at small sizes.  Tracers see the same: the op itself in the forward graph, its *_bwd op in the backward graph.
+def _below_autograd(name, *args):
+    with torch._C._AutoDispatchBelowAutograd():
+        return getattr(torch.ops.xpu_ops, name).default(*args)
 
 
-def _rope_axes_setup(ctx, inputs, output):
-    _, cos, sin, positions, ctx.sections, ctx.interleaved = inputs
-    ctx.has_pos = positions is not None
-    ctx.save_for_backward(cos, sin, *((positions,) if ctx.has_pos else ()))
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
-def _rope_axes_backward(ctx, gy):
-    _refuse_table_grad(ctx, "rope_axes", 1)
-    cos, sin, *pos = ctx.saved_tensors
-    gx = torch.ops.xpu_ops.rope_axes_bwd(gy, cos, sin, pos[0] if pos else None, ctx.sections, ctx.interleaved) if ctx.needs_input_grad[0] else None
-    return gx, None, None, None, None, None
+class _RopeAxes(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, cos, sin, positions, sections, interleaved):
+        ctx.sections, ctx.interleaved = sections, interleaved
+        ctx.save_for_backward(cos, sin, positions)
+        return _below_autograd("rope_axes", x, cos, sin, positions, sections, interleaved)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        return torch.ops.xpu_ops.rope_axes_bwd.default(gy, *ctx.saved_tensors, ctx.sections, ctx.interleaved), None, None, None, None, None
 
 
-def _qk_norm_rope_setup(ctx, inputs, output):
-    q, k, wq, wk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps, _ = inputs
-    ctx.has = [t is not None for t in (wq, wk, positions)]
-    ctx.save_for_backward(q, k, cos, sin, *(t for t in (wq, wk, positions) if t is not None))
+def _rope_axes(x, cos, sin, positions, sections, interleaved=False):
+    if _wants_grad(cos, sin):
+        raise NotImplementedError("xpu_ops::rope_axes: no gradient for the cos / sin tables")
+    if _wants_grad(x):
+        return _RopeAxes.apply(x, cos, sin, positions, sections, interleaved)
+    return _below_autograd("rope_axes", x, cos, sin, positions, sections, interleaved)
 
 
-def _qk_norm_rope_backward(ctx, gq, gk):
-    _refuse_table_grad(ctx, "qk_norm_rope", 4)
-    q, k, cos, sin, *rest = ctx.saved_tensors
-    wq, wk, positions = (rest.pop(0) if has else None for has in ctx.has)
-    want_gw = ctx.needs_input_grad[2] or ctx.needs_input_grad[3]
-    dq, dk, gwq, gwk = torch.ops.xpu_ops.qk_norm_rope_bwd(q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps, want_gw)
-    need = ctx.needs_input_grad
-    return dq, dk, gwq if wq is not None and need[2] else None, gwk if wk is not None and need[3] else None, *((None,) * 7)
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm):
+        ctx.sections, ctx.interleaved, ctx.eps = sections, interleaved, eps
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
+        return _below_autograd("qk_norm_rope", q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gq, gk):
+        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, gwq, gwk = torch.ops.xpu_ops.qk_norm_rope_bwd.default(q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps,
+                                                                      need[2] or need[3])
+        return dq, dk, gwq if need[2] else None, gwk if need[3] else None, None, None, None, None, None, None, None
 
 
-def _linear_attn_setup(ctx, inputs, output):
-    q, k, v, log_decay, state, lengths, ctx.scale = inputs
-    ctx.has = [t is not None for t in (state, lengths)]
-    ctx.save_for_backward(q, k, v, log_decay, *(t for t in (state, lengths) if t is not None))
-    ctx.set_materialize_grads(False)  # an unused output hands over None: no gradient of the final state is read then
+def _qk_norm_rope(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm=False):
+    if _wants_grad(cos, sin):
+        raise NotImplementedError("xpu_ops::qk_norm_rope: no gradient for the cos / sin tables")
+    if _wants_grad(q, k, wq, wk):
+        return _QkNormRope.apply(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
+    return _below_autograd("qk_norm_rope", q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
 
 
-def _linear_attn_backward(ctx, gy, g_state=None):
-    if ctx.needs_input_grad[3]:
+class _LinearAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, log_decay, state, lengths, scale):
+        ctx.scale = scale
+        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
+        ctx.set_materialize_grads(False)  # an unused output hands over None: no gradient of the final state is read then
+        return _below_autograd("linear_attn", q, k, v, log_decay, state, lengths, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy, g_state):
+        if gy is None and g_state is None:
+            return None, None, None, None, None, None, None
+        q, k, v, log_decay, state, lengths = ctx.saved_tensors
+        if gy is None:
+            gy = torch.zeros_like(q)
+        want = ctx.needs_input_grad[4]
+        dq, dk, dv, d_state = torch.ops.xpu_ops.linear_attn_bwd.default(q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want)
+        return dq, dk, dv, None, d_state if want else None, None, None
+
+
+def _linear_attn(q, k, v, log_decay, state, lengths, scale):
+    if _wants_grad(log_decay):
         raise NotImplementedError("xpu_ops::linear_attn: no gradient for log_decay (only q, k, v and the state are differentiable)")
-    if gy is None and g_state is None:
-        return (None,) * 7
-    q, k, v, log_decay, *rest = ctx.saved_tensors
-    state, lengths = (rest.pop(0) if has else None for has in ctx.has)
-    if gy is None:
-        gy = torch.zeros_like(q)
-    want_d_state = state is not None and ctx.needs_input_grad[4]
-    dq, dk, dv, d_state = torch.ops.xpu_ops.linear_attn_bwd(q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want_d_state)
-    return dq, dk, dv, None, d_state if want_d_state else None, None, None
+    if _wants_grad(q, k, v, state):
+        return _LinearAttn.apply(q, k, v, log_decay, state, lengths, scale)
+    return _below_autograd("linear_attn", q, k, v, log_decay, state, lengths, scale)
+
+
+def _linear_attn_step(q, k, v, log_decay, state, scale):
+    if _wants_grad(q, k, v, log_decay, state):
+        raise NotImplementedError("xpu_ops::linear_attn_step: no gradient (the state is updated in place; use linear_attn to train)")
+    return _below_autograd("linear_attn_step", q, k, v, log_decay, state, scale)
 
 
 def _sdpa_setup(ctx, inputs, output):
@@ -480,9 +518,10 @@ def register():
     reg("xpu_ops::dense_glu", _dense_glu_backward, setup_context=_dense_glu_setup)
     reg("xpu_ops::dense_glu_save", _dense_glu_save_backward, setup_context=_dense_glu_save_setup)
     reg("xpu_ops::rope", _rope_backward, setup_context=_rope_setup)
-    reg("xpu_ops::rope_axes", _rope_axes_backward, setup_context=_rope_axes_setup)
-    reg("xpu_ops::qk_norm_rope", _qk_norm_rope_backward, setup_context=_qk_norm_rope_setup)
-    reg("xpu_ops::linear_attn", _linear_attn_backward, setup_context=_linear_attn_setup)
+    from . import ops
+
+    for name, fn in (("rope_axes", _rope_axes), ("qk_norm_rope", _qk_norm_rope), ("linear_attn", _linear_attn), ("linear_attn_step", _linear_attn_step)):
+        ops._library.impl(name, fn, "Autograd")
     reg("xpu_ops::sdpa", _sdpa_backward, setup_context=_sdpa_setup)
     reg("xpu_ops::sdpa_lse", _sdpa_lse_backward, setup_context=_sdpa_lse_setup)
     reg("xpu_ops::sdpa_masked", _sdpa_masked_backward, setup_context=_sdpa_masked_setup)
@@ -493,7 +532,7 @@ def register():
         reg(f"xpu_ops::{op}", backward, setup_context=setup)
     # An op that was traced before (an inference compile earlier in the process) has its dispatch decisions cached
     # on the Python side; a stale entry for the Autograd key would keep sending traces to the "no formula" fallback.
-    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "linear_attn", "sdpa", "sdpa_lse",
+    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "linear_attn", "linear_attn_step", "sdpa", "sdpa_lse",
                  "sdpa_masked", "sdpa_masked_lse", "add_rms_norm", "add_rms_norm_only", "add_layer_norm", "add_layer_norm_only"):
         packet = getattr(torch.ops.xpu_ops, name)
         for overload in packet.overloads():
