@@ -103,18 +103,21 @@ __device__ __forceinline__ float row_sum(float v, int log2) {
   return v;
 }
 
+// cos and sin of a thread's eight pairs; FULL: tables with a column per element, whose halves may differ.
+template <bool FULL>
 struct Turn {
-  float cl[8], ch[8], sl[8], sh[8];
+  float cl[8], sl[8], ch[FULL ? 8 : 1], sh[FULL ? 8 : 1];
+  __device__ __forceinline__ float c_hi(int e) const { return FULL ? ch[e] : cl[e]; }
+  __device__ __forceinline__ float s_hi(int e) const { return FULL ? sh[e] : sl[e]; }
 };
 
 // The table entries of this thread's eight pairs of token (b, s): one row when they share an axis, else the rows of
 // every axis that occurs, picked per pair.
-template <typename T>
-__device__ __forceinline__ void load_turn(const Prep& p, int j, int b, int s, Turn& t) {
+template <typename T, bool FULL>
+__device__ __forceinline__ void load_turn(const Prep& p, int j, int b, int s, Turn<FULL>& t) {
   const uint32_t bits = p.axis_bits[j];
   const int64_t col = 8 * j;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) t.cl[e] = t.ch[e] = t.sl[e] = t.sh[e] = 0.f;
+  const float nan = __builtin_nanf("");
   for (int a = 0; a < p.axes; ++a) {
     uint32_t hit = 0;  // pairs of this axis
 #pragma unroll
@@ -127,24 +130,17 @@ __device__ __forceinline__ void load_turn(const Prep& p, int j, int b, int s, Tu
     }
     const bool bad = p.pos && (row < 0 || row >= p.table_rows);
     const int64_t at = (bad ? 0 : row) * p.table_stride + col;
-    float c[8], n[8], c2[8], n2[8];
-    load8_as<T>(p.cos, at, p.table_f32, c);
-    load8_as<T>(p.sin, at, p.table_f32, n);
-    if (p.half_off) {
-      load8_as<T>(p.cos, at + p.half_off, p.table_f32, c2);
-      load8_as<T>(p.sin, at + p.half_off, p.table_f32, n2);
-    } else {
+    auto pick = [&](const void* table, int64_t from, float (&to)[8]) {
+      float x[8];
+      load8_as<T>(table, from, p.table_f32, x);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) c2[e] = c[e], n2[e] = n[e];
-    }
-    const float nan = __builtin_nanf("");
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const bool mine = (hit >> e) & 1u;
-      t.cl[e] = mine ? (bad ? nan : c[e]) : t.cl[e];
-      t.sl[e] = mine ? (bad ? nan : n[e]) : t.sl[e];
-      t.ch[e] = mine ? (bad ? nan : c2[e]) : t.ch[e];
-      t.sh[e] = mine ? (bad ? nan : n2[e]) : t.sh[e];
+      for (int e = 0; e < 8; ++e) to[e] = (hit >> e) & 1u ? (bad ? nan : x[e]) : to[e];
+    };
+    pick(p.cos, at, t.cl);
+    pick(p.sin, at, t.sl);
+    if constexpr (FULL) {
+      pick(p.cos, at + p.half_off, t.ch);
+      pick(p.sin, at + p.half_off, t.sh);
     }
   }
 }
@@ -157,7 +153,7 @@ __device__ __forceinline__ void columns(const Prep& p, int j, int& lo, int& hi, 
   hi = rotated ? (p.R >> 1) + 8 * j : lo + 8;
 }
 
-template <typename T, bool NORM, int kHeads>
+template <typename T, bool NORM, bool FULL, int kHeads>
 __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
   typedef typename Eight<T>::type V8;
   const int j = threadIdx.x & ((1 << p.tpr_log2) - 1);
@@ -181,22 +177,22 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
   for (int i = 0; i < kHeads; ++i) {
     if (live && h0 + i < sd.H) {
       const T* row = x + (int64_t)(h0 + i) * sd.xs[1];
-      lo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(row + lo_c));
-      hi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(row + hi_c));
+      lo[i] = *reinterpret_cast<const V8*>(row + lo_c);
+      hi[i] = *reinterpret_cast<const V8*>(row + hi_c);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) lo[i][e] = hi[i][e] = (T)0.f;
     }
   }
-  Turn t;
+  Turn<FULL> t{};
   if (live && rotated) {
-    load_turn<T>(p, j, b, s, t);
+    load_turn<T, FULL>(p, j, b, s, t);
     if (p.transpose) {  // the transposed rotation is the rotation by the tables (c, -s) with the halves of s swapped
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float l = t.sl[e];
-        t.sl[e] = -t.sh[e];
-        t.sh[e] = -l;
+        t.sl[e] = -t.s_hi(e);
+        if constexpr (FULL) t.sh[e] = -l;
       }
     }
   }
@@ -239,7 +235,7 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         ol[e] = from_f32<T>(xl[e] * t.cl[e] - xh[e] * t.sl[e]);
-        oh[e] = from_f32<T>(xh[e] * t.ch[e] + xl[e] * t.sh[e]);
+        oh[e] = from_f32<T>(xh[e] * t.c_hi(e) + xl[e] * t.s_hi(e));
       }
     } else {
 #pragma unroll
@@ -253,7 +249,7 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
 
 // Backward of norm + rotation.  A block walks the units (token, group of heads) of one side; a lane keeps the same
 // columns throughout, so its share of the weight gradient stays in registers and leaves as one row per block.
-template <typename T, int kHeads>
+template <typename T, bool FULL, int kHeads>
 __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
   typedef typename Eight<T>::type V8;
   __shared__ float red[4096];
@@ -291,17 +287,17 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
       if (live && h0 + i < sd.H) {
         const T* xr = x + (int64_t)(h0 + i) * sd.xs[1];
         const T* gr = g + (int64_t)(h0 + i) * sd.gs[1];
-        xlo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(xr + lo_c));
-        xhi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(xr + hi_c));
-        glo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(gr + lo_c));
-        ghi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(gr + hi_c));
+        xlo[i] = *reinterpret_cast<const V8*>(xr + lo_c);
+        xhi[i] = *reinterpret_cast<const V8*>(xr + hi_c);
+        glo[i] = *reinterpret_cast<const V8*>(gr + lo_c);
+        ghi[i] = *reinterpret_cast<const V8*>(gr + hi_c);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) xlo[i][e] = xhi[i][e] = glo[i][e] = ghi[i][e] = (T)0.f;
       }
     }
-    Turn t;
-    if (live && rotated) load_turn<T>(p, j, b, s, t);
+    Turn<FULL> t{};
+    if (live && rotated) load_turn<T, FULL>(p, j, b, s, t);
 #pragma unroll
     for (int i = 0; i < kHeads; ++i) {
       float xl[8], xh[8], gl[8], gh[8];
@@ -309,8 +305,8 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
       for (int e = 0; e < 8; ++e) {
         xl[e] = to_f32(xlo[i][e]), xh[e] = to_f32(xhi[i][e]);
         const float a = to_f32(glo[i][e]), c = to_f32(ghi[i][e]);
-        gl[e] = rotated ? a * t.cl[e] + c * t.sh[e] : a;
-        gh[e] = rotated ? c * t.ch[e] - a * t.sl[e] : c;
+        gl[e] = rotated ? a * t.cl[e] + c * t.s_hi(e) : a;
+        gh[e] = rotated ? c * t.c_hi(e) - a * t.sl[e] : c;
       }
       if (!live) {
 #pragma unroll
@@ -355,11 +351,11 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
   }
 }
 
-// gw[c] = sum over a side's partial rows, in a fixed order: 16 columns x 16 row lanes per block, block (c/16, side).
+// gw[c] = sum over a side's partial rows, in a fixed order: 16 columns x 64 row lanes per block, block (c/16, side).
 template <typename WT>
-__global__ __launch_bounds__(256) void gw_sum_kernel(const float* __restrict__ part, int blocks0, int blocks1, int D, WT* __restrict__ gw0,
-                                                     WT* __restrict__ gw1) {
-  __shared__ float red[16][17];
+__global__ __launch_bounds__(1024) void gw_sum_kernel(const float* __restrict__ part, int blocks0, int blocks1, int D, WT* __restrict__ gw0,
+                                                      WT* __restrict__ gw1) {
+  __shared__ float red[64][17];
   const bool second = blockIdx.y != 0;
   WT* gw = second ? gw1 : gw0;
   if (gw == nullptr) return;
@@ -368,15 +364,18 @@ __global__ __launch_bounds__(256) void gw_sum_kernel(const float* __restrict__ p
   const int rows = second ? blocks1 : blocks0;
   const float* src = part + (second ? (int64_t)blocks0 * D : 0) + col;
   float a = 0.f;
-  for (int r = l; r < rows; r += 16) a += src[(int64_t)r * D];
+#pragma unroll 8
+  for (int r = l; r < rows; r += 64) a += src[(int64_t)r * D];
   red[l][c] = a;
   __syncthreads();
-  if (l == 0) {
+  if (l < 4) {  // four lanes of a column add sixteen rows each, then one of them the four
     float t = 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) t += red[i][c];
-    gw[col] = from_f32<WT>(t);
+    for (int i = 0; i < 16; ++i) t += red[16 * l + i][c];
+    red[16 * l][c] = t;
   }
+  __syncthreads();
+  if (l == 0) gw[col] = from_f32<WT>((red[0][c] + red[16][c]) + (red[32][c] + red[48][c]));
 }
 
 // ------------------------------------------------------------------ host side
@@ -464,33 +463,40 @@ int check_sizes(int64_t B, int64_t H0, int64_t H1, int64_t S, int64_t D, int dty
   return XG_OK;
 }
 
-template <typename T, bool NORM, int kHeads>
+template <typename T, bool NORM, bool FULL, int kHeads>
 int launch_prep(Prep& p, int64_t tokens, hipStream_t stream) {
   for (Side& sd : p.side) sd.chunks = (sd.H + kHeads - 1) / kHeads;
   p.n_chunks = (uint32_t)(p.side[0].chunks + p.side[1].chunks);
   p.by_chunks = FastDiv(p.n_chunks);
   p.units = (uint32_t)(tokens * p.n_chunks);
   const uint32_t per_block = 256u >> p.tpr_log2;
-  hipLaunchKernelGGL((prep_kernel<T, NORM, kHeads>), dim3((p.units + per_block - 1) / per_block), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((prep_kernel<T, NORM, FULL, kHeads>), dim3((p.units + per_block - 1) / per_block), dim3(256), 0, stream, p);
   return status_from_hip(hipGetLastError());
 }
 
 template <bool NORM>
 int run_prep(Prep& p, int64_t tokens, int dtype, hipStream_t stream) {
-  auto go = [&](auto heads) {
+  auto go = [&](auto full, auto heads) {
+    constexpr bool FULL = decltype(full)::value;
     constexpr int kHeads = decltype(heads)::value;
-    if (dtype == XG_BF16) return launch_prep<bf16_t, NORM, kHeads>(p, tokens, stream);
-    if (dtype == XG_F16) return launch_prep<f16_t, NORM, kHeads>(p, tokens, stream);
-    return launch_prep<float, NORM, kHeads>(p, tokens, stream);
+    if (dtype == XG_BF16) return launch_prep<bf16_t, NORM, FULL, kHeads>(p, tokens, stream);
+    if (dtype == XG_F16) return launch_prep<f16_t, NORM, FULL, kHeads>(p, tokens, stream);
+    return launch_prep<float, NORM, FULL, kHeads>(p, tokens, stream);
   };
-  // Four heads a thread share one read of the tables; few rows are spread over as many threads as there are.
+  // Several heads a thread share one read of the tables (8 without the norm, 4 with it, whose weights and sums take
+  // registers); few rows are spread over as many threads as there are.
   const int64_t threads = (tokens * (p.side[0].H + p.side[1].H)) << p.tpr_log2;
-  return threads >= 4 * 256 * 1024 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 1>{});
+  constexpr int kMany = NORM ? 4 : 8;
+  const std::integral_constant<int, kMany> many;
+  const std::integral_constant<int, 1> one;
+  if (threads >= 4 * 256 * 1024) return p.half_off ? go(std::true_type{}, many) : go(std::false_type{}, many);
+  return p.half_off ? go(std::true_type{}, one) : go(std::false_type{}, one);
 }
 
 constexpr int kBwdHeads = 2;
 
-// Blocks of the two sides of the backward: as many as the chip holds at once, in proportion to the rows.
+// Blocks of the two sides of the backward, in proportion to the rows: as many as the chip holds at once (three per compute
+// unit by registers; B4 S2048 H32/32 D128 bf16: 80.7 us with 768, 84 with 1536, 101 with 1024, 4.99 TB/s).
 void bwd_blocks(int64_t tokens, int64_t H0, int64_t H1, int64_t D, int& n0, int& n1) {
   int log2 = 0;
   while ((1 << log2) < D / 16) ++log2;
@@ -498,7 +504,7 @@ void bwd_blocks(int64_t tokens, int64_t H0, int64_t H1, int64_t D, int& n0, int&
   auto count = [&](int64_t H) {
     if (H == 0 || tokens == 0) return (int64_t)0;
     const int64_t units = tokens * ((H + kBwdHeads - 1) / kBwdHeads);
-    const int64_t most = 1024 * H / (H0 + H1);
+    const int64_t most = 768 * H / (H0 + H1);
     const int64_t want = (units + per_block - 1) / per_block;
     return want < (most < 1 ? 1 : most) ? want : (most < 1 ? 1 : most);
   };
@@ -577,18 +583,22 @@ extern "C" int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w
   p.blocks0 = n0;
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(n0 + n1), block(256);
-  if (dtype == XG_BF16)
-    hipLaunchKernelGGL((prep_bwd_kernel<bf16_t, kBwdHeads>), grid, block, 0, st, p);
-  else if (dtype == XG_F16)
-    hipLaunchKernelGGL((prep_bwd_kernel<f16_t, kBwdHeads>), grid, block, 0, st, p);
-  else
-    hipLaunchKernelGGL((prep_bwd_kernel<float, kBwdHeads>), grid, block, 0, st, p);
+  auto go = [&](auto full) {
+    constexpr bool FULL = decltype(full)::value;
+    if (dtype == XG_BF16)
+      hipLaunchKernelGGL((prep_bwd_kernel<bf16_t, FULL, kBwdHeads>), grid, block, 0, st, p);
+    else if (dtype == XG_F16)
+      hipLaunchKernelGGL((prep_bwd_kernel<f16_t, FULL, kBwdHeads>), grid, block, 0, st, p);
+    else
+      hipLaunchKernelGGL((prep_bwd_kernel<float, FULL, kBwdHeads>), grid, block, 0, st, p);
+  };
+  p.half_off ? go(std::true_type{}) : go(std::false_type{});
   if (hipGetLastError() != hipSuccess) return XG_ERR_LAUNCH;
   if (!want_gw) return XG_OK;
   const dim3 sum_grid((unsigned)(D / 16), 2);
   auto sum = [&](auto zero) {
     typedef decltype(zero) WT;
-    hipLaunchKernelGGL((gw_sum_kernel<WT>), sum_grid, block, 0, st, workspace, n0, n1, (int)D, (WT*)gw_q, (WT*)gw_k);
+    hipLaunchKernelGGL((gw_sum_kernel<WT>), sum_grid, dim3(1024), 0, st, workspace, n0, n1, (int)D, (WT*)gw_q, (WT*)gw_k);
   };
   if (w_dtype == XG_F32)
     sum(0.f);
