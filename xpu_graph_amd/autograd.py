@@ -286,9 +286,17 @@ def _rope_backward(ctx, gy):
 # The three ops below go through torch.autograd.Function at the Autograd dispatch key instead of register_autograd: the
 # bookkeeping of the latter (defaults, metadata and pytrees of every call) costs 15 to 30 us a call, more than their kernels take
 # at small sizes.  Tracers see the same: the op itself in the forward graph, its *_bwd op in the backward graph.
-def _below_autograd(name, *args):
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _below_autograd(name, first, *args):
+    """The op without its autograd formula.  Plain GPU tensors go straight to what the dispatcher would call."""
+    if first.__class__ in _PLAIN and first.is_cuda and not torch._C._len_torch_dispatch_stack() and torch._C._functorch.peek_interpreter_stack() is None:
+        from . import ops
+
+        return getattr(ops, "_" + name)(first, *args)
     with torch._C._AutoDispatchBelowAutograd():
-        return getattr(torch.ops.xpu_ops, name).default(*args)
+        return getattr(torch.ops.xpu_ops, name).default(first, *args)
 
 
 def _wants_grad(*tensors):
@@ -305,7 +313,7 @@ class _RopeAxes(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, gy):
-        return torch.ops.xpu_ops.rope_axes_bwd.default(gy, *ctx.saved_tensors, ctx.sections, ctx.interleaved), None, None, None, None, None
+        return _below_autograd("rope_axes_bwd", gy, *ctx.saved_tensors, ctx.sections, ctx.interleaved), None, None, None, None, None
 
 
 def _rope_axes(x, cos, sin, positions, sections, interleaved=False):
@@ -328,8 +336,8 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, gq, gk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         need = ctx.needs_input_grad
-        dq, dk, gwq, gwk = torch.ops.xpu_ops.qk_norm_rope_bwd.default(q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps,
-                                                                      need[2] or need[3])
+        dq, dk, gwq, gwk = _below_autograd("qk_norm_rope_bwd", q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps,
+                                           need[2] or need[3])
         return dq, dk, gwq if need[2] else None, gwk if need[3] else None, None, None, None, None, None, None, None
 
 
@@ -358,7 +366,7 @@ class _LinearAttn(torch.autograd.Function):
         if gy is None:
             gy = torch.zeros_like(q)
         want = ctx.needs_input_grad[4]
-        dq, dk, dv, d_state = torch.ops.xpu_ops.linear_attn_bwd.default(q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want)
+        dq, dk, dv, d_state = _below_autograd("linear_attn_bwd", q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want)
         return dq, dk, dv, None, d_state if want else None, None, None
 
 
