@@ -73,7 +73,6 @@ struct Params {
   int len64;
   int B, H, S;
   int n_seg, seg_chunks;
-  int stages;               // chunks in LDS
 };
 
 // Row of an accumulator tile (or lane of an operand) -> row of S, column of V: bits 2 and 3 change places.
@@ -130,27 +129,51 @@ __device__ __forceinline__ f32x16 mma_parts(const Parts<NA>& a, const Parts<NB>&
   return c;
 }
 
-// A chunk's rows of one operand in LDS: [32][D], 16-byte pieces swizzled for both kinds of reads.
+// A chunk's rows of one operand in LDS: [32][D], 16-byte pieces swizzled for both kinds of reads.  The addresses of a lane's
+// reads are kept in registers; which tile and stage they go to is an immediate offset.
 template <typename T, int D>
 struct Tile {
   static constexpr int RB = D * 2;
   static constexpr int BYTES = C * RB;
   typedef typename Vec8<T>::type V8;
+  typedef __attribute__((address_space(3))) const V8 lds_V8;
 
-  // row `row`, columns 16 t + 8 h .. +7
-  __device__ static __forceinline__ V8 row_frag(const char* tile, int row, int t, int h) {
-    return *reinterpret_cast<const V8*>(tile + row * RB + (((2 * t + h) ^ swz_v<D>(row)) << 4));
+  // row lane % 32, columns 16 t + 8 h .. +7
+  __device__ static __forceinline__ uint32_t row_address(uint32_t lds, int t, int lane) {
+    const int row = lane & 31, h = lane >> 5;
+    return lds + row * RB + (((2 * t + h) ^ swz_v<D>(row)) << 4);
   }
-  // column 32 ct + sigma(lane % 32), rows 16 t + 4 h .. +3 and 16 t + 8 + 4 h .. +3: two transposing reads, in which sixteen lanes
-  // address four rows of four 8-byte pieces and lane i of them receives column i; the middle pieces are swapped
-  __device__ static __forceinline__ V8 col_frag(const char* tile, int ct, int t, int lane) {
+  __device__ static __forceinline__ V8 row_frag(uint32_t at) { return *(lds_V8*)at; }
+  // column 32 ct + sigma(lane % 32), rows 4 h .. +3 (hi: 8 + 4 h .. +3) of sixteen: a transposing read, in which sixteen lanes address
+  // four rows of four 8-byte pieces and lane i of them receives column i; the middle pieces are swapped
+  __device__ static __forceinline__ uint32_t col_address(uint32_t lds, int ct, int hi, int lane) {
     const int h = lane >> 5, a16 = lane & 15, b16 = (lane >> 4) & 1;
     const int piece = ((a16 & 1) << 1) | ((a16 >> 1) & 1);
-    const int row = 16 * t + 4 * h + (a16 >> 2), ch = 4 * ct + 2 * b16 + (piece >> 1), sub = (piece & 1) << 3;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (row + 8) * RB + ((ch ^ swz_v<D>(row + 8)) << 4) + sub));
+    const int row = 8 * hi + 4 * h + (a16 >> 2), ch = 4 * ct + 2 * b16 + (piece >> 1), sub = (piece & 1) << 3;
+    return lds + row * RB + ((ch ^ swz_v<D>(row)) << 4) + sub;
+  }
+  __device__ static __forceinline__ V8 col_frag(uint32_t lo_at, uint32_t hi_at) {
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)lo_at);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)hi_at);
     const s16x8 both = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     return __builtin_bit_cast(V8, both);
+  }
+};
+
+// The addresses of a wave's transposing reads of K (every column) and of V (its own 32).
+template <typename T, int D>
+struct ColAddresses {
+  uint32_t k_lo[D / 32], k_hi[D / 32], v_lo, v_hi;
+  __device__ __forceinline__ ColAddresses(uint32_t k_tile, uint32_t v_tile, int w, int lane) {
+#pragma unroll
+    for (int dt = 0; dt < D / 32; ++dt) {
+      k_lo[dt] = Tile<T, D>::col_address(k_tile, dt, 0, lane);
+      k_hi[dt] = Tile<T, D>::col_address(k_tile, dt, 1, lane);
+      asm volatile("" : "+v"(k_lo[dt]), "+v"(k_hi[dt]));  // held, not recomputed
+    }
+    v_lo = Tile<T, D>::col_address(v_tile, w, 0, lane);
+    v_hi = Tile<T, D>::col_address(v_tile, w, 1, lane);
+    asm volatile("" : "+v"(v_lo), "+v"(v_hi));
   }
 };
 
@@ -175,21 +198,18 @@ __device__ __forceinline__ uint32_t lds_address(const char* at) {
   return __builtin_amdgcn_readfirstlane(x);
 }
 
-// One operand's chunks on their way from global memory to LDS.
+// One operand's chunks on their way from global memory to LDS, in order.
 template <typename T, int D>
 struct Mover {
-  static constexpr int NT = D * 2;             // threads: D/32 waves
   static constexpr int RB = D * 2;
-  const char* first;                           // token 0 in the order of the recurrence
+  const char* next;                            // the lowest address of the next whole chunk
   int64_t row_bytes;                           // signed: a reversed operand walks backwards
-  uint32_t off[2];                             // this lane's part of the tile, from its lowest address
-  int64_t low;                                 // from the address of a chunk's first token to its lowest
+  uint32_t off[2];                             // this lane's part of a tile, from its lowest address
 
-  __device__ __forceinline__ void bind(const Operand& o, int b, int head, int len, int reverse, int tid) {
-    const int64_t last = reverse ? (int64_t)(len - 1) * o.s[2] : 0;
-    first = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (head / o.group) * o.s[1] + last) * 2;
+  __device__ __forceinline__ void bind(const Operand& o, int b, int head, int len, int reverse, int t0, int tid) {
     row_bytes = (reverse ? -o.s[2] : o.s[2]) * 2;
-    low = reverse ? (C - 1) * row_bytes : 0;
+    const int64_t lowest = reverse ? (int64_t)(len - 1 - t0) - (C - 1) : (int64_t)t0;
+    next = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (head / o.group) * o.s[1] + lowest * o.s[2]) * 2;
     const uint32_t pitch = (uint32_t)(o.s[2] * 2);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -200,20 +220,23 @@ struct Mover {
   // bytes [1024 (2 wave + i) + 16 lane, + 16) of a tile
   __device__ static __forceinline__ int place(int tid, int i) { return (2 * (tid >> 6) + i) * 1024 + (tid & 63) * 16; }
 
-  // 32 whole tokens from t0 on, straight to LDS (waits by vmcnt)
-  __device__ __forceinline__ void load(int t0, const char* tile, int w) const {
-    const uint64_t base = (uint64_t)(uintptr_t)(first + (int64_t)t0 * row_bytes + low);  // the same for every lane
+  // 32 whole tokens straight to LDS (waits by vmcnt); `to`: this wave's place in the tile
+  __device__ __forceinline__ void load(uint32_t to) {
+    const uint64_t base = (uint64_t)(uintptr_t)next;  // the same for every lane
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)base), hi = __builtin_amdgcn_readfirstlane((uint32_t)(base >> 32));
-#pragma unroll
-    for (int i = 0; i < 2; ++i) load_to_lds16((const void*)(uintptr_t)((uint64_t)hi << 32 | lo), off[i], lds_address(tile + (2 * w + i) * 1024));
+    const void* from = (const void*)(uintptr_t)((uint64_t)hi << 32 | lo);
+    load_to_lds16(from, off[0], to);
+    load_to_lds16(from, off[1], to + 1024);
+    next += C * row_bytes;
   }
-  // n < 32 tokens, zeros behind them
-  __device__ __forceinline__ void load_tail(int t0, int n, char* tile, int tid) const {
+  // the last n < 32 tokens, zeros behind them
+  __device__ __forceinline__ void load_tail(int n, char* tile, int tid) const {
+    const char* first = next + (row_bytes < 0 ? -(C - 1) * row_bytes : 0);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int pos = place(tid, i), row = pos / RB, pc = (pos % RB) >> 4;
       u32x4 x = {0, 0, 0, 0};
-      if (row < n) x = *reinterpret_cast<const u32x4*>(first + (int64_t)(t0 + row) * row_bytes + ((pc ^ swz_v<D>(row)) << 4));
+      if (row < n) x = *reinterpret_cast<const u32x4*>(first + row * row_bytes + ((pc ^ swz_v<D>(row)) << 4));
       *reinterpret_cast<u32x4*>(tile + pos) = x;
     }
   }
@@ -228,15 +251,15 @@ __device__ __forceinline__ void chunk_barrier() {
 
 // S += sum_j x_j k_j on this wave's 32 columns, x[t][jj] the weighed value of the token in slot jj of k-step t.
 // Three bf16 parts of x where the state is a result (`whole`), two where it only feeds O.
-template <typename T, int D>
-__device__ __forceinline__ void add_to_state(f32x16 (&S)[D / 32], const char* k_tile, float (&x)[2][8], bool whole, int lane) {
+template <typename T, int D, int AT>
+__device__ __forceinline__ void add_to_state(f32x16 (&S)[D / 32], const ColAddresses<T, D>& at, float (&x)[2][8], bool whole) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const Parts<2> xv = split<2>(x[t]);
     Parts<kParts<T>> kf[D / 32];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
-      kf[dt] = as_parts<T>(Tile<T, D>::col_frag(k_tile, dt, t, lane));
+      kf[dt] = as_parts<T>(Tile<T, D>::col_frag(at.k_lo[dt] + AT + 16 * t * Tile<T, D>::RB, at.k_hi[dt] + AT + 16 * t * Tile<T, D>::RB));
       S[dt] = mma_parts(kf[dt], xv, S[dt]);
     }
     if (whole) {
@@ -296,28 +319,36 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
     for (int i = 0; i < 16; ++i) S[dt][i] = 0.f;
   Mover<T, D> km, vm;
-  km.bind(pr.k, b, head, len, pr.reverse, tid);
-  vm.bind(pr.v, b, head, len, pr.reverse, tid);
+  km.bind(pr.k, b, head, len, pr.reverse, t0, tid);
+  vm.bind(pr.v, b, head, len, pr.reverse, t0, tid);
   float f[2][8];
   token_factors(f, g2, C, pr.e, pr.s_state, h);
-  km.load(t0, smem, w);
-  vm.load(t0, smem + TL::BYTES, w);
-  for (int stage = 0; t0 < t_end; t0 += C, stage ^= 1) {
+  const uint32_t lds = lds_address(smem);
+  const ColAddresses<T, D> at(lds, lds + TL::BYTES, w, lane);
+  auto issue = [&](uint32_t stage_at) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds + stage_at + 2048 * w);
+    km.load(to);
+    vm.load(to + TL::BYTES);
+  };
+  issue(0);
+  auto step = [&](auto stage) {
+    constexpr int AT = decltype(stage)::value * STAGE;
     chunk_barrier<0>();
-    if (t0 + C < t_end) {
-      km.load(t0 + C, smem + (stage ^ 1) * STAGE, w);
-      vm.load(t0 + C, smem + (stage ^ 1) * STAGE + TL::BYTES, w);
-    }
-    const char* k_s = smem + stage * STAGE;
+    if (t0 + C < t_end) issue(STAGE - AT);
     const float rest = decay(g2, t_end - t0 - C);
     float x[2][8];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const typename TL::V8 vf = TL::col_frag(k_s + TL::BYTES, w, t, lane);
+      const typename TL::V8 vf = TL::col_frag(at.v_lo + AT + 16 * t * TL::RB, at.v_hi + AT + 16 * t * TL::RB);
 #pragma unroll
       for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[jj] * (f[t][jj] * rest);
     }
-    add_to_state<T, D>(S, k_s, x, true, lane);
+    add_to_state<T, D, AT>(S, at, x, true);
+    t0 += C;
+  };
+  while (t0 < t_end) {
+    step(std::integral_constant<int, 0>{});
+    if (t0 < t_end) step(std::integral_constant<int, 1>{});
   }
   float* to = pr.seg_states + ((int64_t)bh * p.n_seg + seg) * (D * D);
 #pragma unroll
@@ -368,7 +399,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   typedef Tile<T, D> TL;
   constexpr int OP = kParts<T>;  // parts of S and P as operands of O
   constexpr int STAGE = 3 * TL::BYTES;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // stages of Q, K, V
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of Q, K, V
   const Problem& pr = p.pr[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -432,26 +463,25 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 
   if (t_beg < t_end) {
     Mover<T, D> qm, km, vm;
-    qm.bind(pr.q, b, head, len, pr.reverse, tid);
-    km.bind(pr.k, b, head, len, pr.reverse, tid);
-    vm.bind(pr.v, b, head, len, pr.reverse, tid);
-    auto issue = [&](int t0, int stage) {
-      if (t0 >= t_end) return;
-      char* to = smem + stage * STAGE;
+    qm.bind(pr.q, b, head, len, pr.reverse, t_beg, tid);
+    km.bind(pr.k, b, head, len, pr.reverse, t_beg, tid);
+    vm.bind(pr.v, b, head, len, pr.reverse, t_beg, tid);
+    const uint32_t lds = lds_address(smem);
+    auto issue = [&](int t0, int stage_at) {
       if (t_end - t0 >= C) {
-        qm.load(t0, to, w);
-        km.load(t0, to + TL::BYTES, w);
-        vm.load(t0, to + 2 * TL::BYTES, w);
+        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + stage_at + 2048 * w);
+        qm.load(to);
+        km.load(to + TL::BYTES);
+        vm.load(to + 2 * TL::BYTES);
       } else {
-        qm.load_tail(t0, t_end - t0, to, tid);
-        km.load_tail(t0, t_end - t0, to + TL::BYTES, tid);
-        vm.load_tail(t0, t_end - t0, to + 2 * TL::BYTES, tid);
+        qm.load_tail(t_end - t0, smem + stage_at, tid);
+        km.load_tail(t_end - t0, smem + stage_at + TL::BYTES, tid);
+        vm.load_tail(t_end - t0, smem + stage_at + 2 * TL::BYTES, tid);
       }
     };
-    const int ahead = p.stages - 1;  // chunks in flight: one or two
-    for (int i = 0; i < ahead; ++i) issue(t_beg + i * C, i);
+    issue(t_beg, 0);
 
-    // factors that do not change from chunk to chunk
+    // what does not change from chunk to chunk: factors, addresses
     float f[2][8];
     token_factors(f, g2, C, pr.e, pr.s_state, h);
     const float row_f = decay(g2, l32 + 1 - pr.e) * pr.s_inter;
@@ -461,20 +491,24 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       const int d = l32 - (8 * (i >> 2) + 4 * h + (i & 3));
       p_f[i] = d < 0 ? 0.f : decay(g2, d) * pr.s_intra;
     }
+    const float lam_c = decay(g2, C);
+    const ColAddresses<T, D> at(lds + TL::BYTES, lds + 2 * TL::BYTES, w, lane);
+    uint32_t row_at[D / 16];
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) {
+      row_at[t] = TL::row_address(lds, t, lane);
+      asm volatile("" : "+v"(row_at[t]));
+    }
+    // lane: query l32, columns 32 w + 16 t + 8 h .. +7 in registers 8 t .. 8 t + 7
+    const int out_size = pr.out_f32 ? 4 : 2;
+    const int64_t out_row = (pr.reverse ? -pr.os[2] : pr.os[2]) * out_size;
+    char* out = reinterpret_cast<char*>(pr.out) + (out0 + (int64_t)(pr.reverse ? len - 1 - t_beg : t_beg) * pr.os[2] + 32 * w + 8 * h) * out_size + l32 * out_row;
 
-    int stage = 0;
-    for (int t0 = t_beg; t0 < t_end; t0 += C, stage = stage == ahead ? 0 : stage + 1) {
+    auto step = [&](auto stage, int t0) {
+      constexpr int AT = decltype(stage)::value * STAGE;
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      if (ahead == 1 || t0 + C >= t_end)
-        chunk_barrier<0>();
-      else if (t0 < t_beg + 2 * C)  // the next chunk's six loads have been issued since
-        chunk_barrier<6>();
-      else  // and the stores (two or more) of one chunk at least
-        chunk_barrier<8>();
-      issue(t0 + ahead * C, stage == 0 ? ahead : stage - 1);
-      const char* q_s = smem + stage * STAGE;
-      const char* k_s = q_s + TL::BYTES;
-      const char* v_s = q_s + 2 * TL::BYTES;
+      chunk_barrier<0>();
+      if (t0 + C < t_end) issue(t0 + C, STAGE - AT);
 
       // P^T = K Q^T and O^T = S^T Q^T from the same rows of Q; each query of O scaled by its decay
       f32x16 P, O;
@@ -482,8 +516,8 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       for (int i = 0; i < 16; ++i) P[i] = O[i] = 0.f;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        const V8 qf = TL::row_frag(q_s, l32, t, h);
-        P = mma(TL::row_frag(k_s, l32, t, h), qf, P);
+        const V8 qf = TL::row_frag(row_at[t] + AT);
+        P = mma(TL::row_frag(row_at[t] + AT + TL::BYTES), qf, P);
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = S[t >> 1][8 * (t & 1) + i];
@@ -492,7 +526,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       O *= row_f;
       V8 vf[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(v_s, w, t, lane);
+      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(at.v_lo + AT + 16 * t * TL::RB, at.v_hi + AT + 16 * t * TL::RB);
 
       // O^T += V^T P^T
 #pragma unroll
@@ -503,17 +537,14 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         O = mma_parts(as_parts<T>(vf[t]), split<OP>(x), O);
       }
 
-      // lane: query l32, columns 32 w + 16 t + 8 h .. +7 in registers 8 t .. 8 t + 7
       if (l32 < n) {
-        const int64_t token = pr.reverse ? (int64_t)len - 1 - (t0 + l32) : (int64_t)t0 + l32;
-        const int64_t at = out0 + token * pr.os[2] + 32 * w + 8 * h;
         if (pr.out_f32) {
-          float* o = reinterpret_cast<float*>(pr.out) + at;
+          float* o = reinterpret_cast<float*>(out);
 #pragma unroll
           for (int g = 0; g < 4; ++g)
             *reinterpret_cast<f32x4*>(o + 16 * (g >> 1) + 4 * (g & 1)) = f32x4{O[4 * g], O[4 * g + 1], O[4 * g + 2], O[4 * g + 3]};
         } else {
-          T* o = reinterpret_cast<T*>(pr.out) + at;
+          T* o = reinterpret_cast<T*>(out);
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             V8 y;
@@ -523,10 +554,14 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
           }
         }
       }
+      out += C * out_row;
 
       if (t0 + C < t_end || keep_state) {
-        if (n < C) token_factors(f, g2, n, pr.e, pr.s_state, h);
-        const float lam_n = decay(g2, n);
+        float lam_n = lam_c;
+        if (n < C) {
+          token_factors(f, g2, n, pr.e, pr.s_state, h);
+          lam_n = decay(g2, n);
+        }
 #pragma unroll
         for (int dt = 0; dt < D / 32; ++dt) S[dt] *= lam_n;
         float x[2][8];
@@ -534,8 +569,12 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[t][jj] * f[t][jj];
-        add_to_state<T, D>(S, k_s, x, keep_state, lane);
+        add_to_state<T, D, AT>(S, at, x, keep_state);
       }
+    };
+    for (int t0 = t_beg; t0 < t_end; t0 += 2 * C) {
+      step(std::integral_constant<int, 0>{}, t0);
+      if (t0 + C < t_end) step(std::integral_constant<int, 1>{}, t0 + C);
     }
   }
 
@@ -685,15 +724,12 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
-  auto kernel = linear_attn_kernel<T, D>;
-  constexpr int STAGE = 3 * Tile<T, D>::BYTES;
-  if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 3 * STAGE)) return rc;
   const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), block(D * 2);
   if (p.n_seg > 1) {
     hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, block, 0, st, p);
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
   }
-  hipLaunchKernelGGL(kernel, grid, block, p.stages * STAGE, st, p);
+  hipLaunchKernelGGL((linear_attn_kernel<T, D>), grid, block, 0, st, p);
   return status_from_hip(hipGetLastError());
 }
 
@@ -736,7 +772,6 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
   p.H = (int)H;
   p.S = (int)S;
   segments(B * H, 1, S, p.n_seg, p.seg_chunks);
-  p.stages = p.n_seg > 1 ? 2 : 3;
   if (p.n_seg > 1) {
     if (!workspace) return XG_ERR_NULL_PTR;
     if (workspace_floats < B * H * p.n_seg * D * D) return XG_ERR_BAD_ARG;
@@ -786,7 +821,6 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   p.H = (int)H;
   p.S = (int)S;
   segments(B * H, 3, S, p.n_seg, p.seg_chunks);
-  p.stages = p.n_seg > 1 ? 2 : 3;
   const int64_t need = xg_linear_attn_bwd_workspace_floats(B, H, Hkv, S, D);
   if (need) {
     if (!workspace) return XG_ERR_NULL_PTR;
