@@ -393,13 +393,14 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
   }
 }
 
-template <typename T, int D>
+// STAGES: chunks of tiles in LDS.
+template <typename T, int D, int STAGES>
 __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_attn_kernel(const Params p) {
   typedef typename Vec8<T>::type V8;
   typedef Tile<T, D> TL;
   constexpr int OP = kParts<T>;  // parts of S and P as operands of O
   constexpr int STAGE = 3 * TL::BYTES;
-  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of Q, K, V
+  extern __shared__ __attribute__((aligned(1024))) char smem[];  // stages of Q, K, V
   const Problem& pr = p.pr[blockIdx.y];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -480,6 +481,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       }
     };
     issue(t_beg, 0);
+    if (STAGES > 2 && t_beg + C < t_end) issue(t_beg + C, STAGE);
 
     // what does not change from chunk to chunk: factors, addresses
     float f[2][8];
@@ -507,8 +509,13 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     auto step = [&](auto stage, int t0) {
       constexpr int AT = decltype(stage)::value * STAGE;
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      chunk_barrier<0>();
-      if (t0 + C < t_end) issue(t0 + C, STAGE - AT);
+      if (STAGES == 2 || t0 + C >= t_end)
+        chunk_barrier<0>();
+      else if (t0 < t_beg + 2 * C)  // the next chunk's six loads have been issued since
+        chunk_barrier<6>();
+      else  // and the stores (two or more) of one chunk at least
+        chunk_barrier<8>();
+      if (t0 + (STAGES - 1) * C < t_end) issue(t0 + (STAGES - 1) * C, (AT + (STAGES - 1) * STAGE) % (STAGES * STAGE));
 
       // P^T = K Q^T and O^T = S^T Q^T from the same rows of Q; each query of O scaled by its decay
       f32x16 P, O;
@@ -572,9 +579,11 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         add_to_state<T, D, AT>(S, at, x, keep_state);
       }
     };
-    for (int t0 = t_beg; t0 < t_end; t0 += 2 * C) {
-      step(std::integral_constant<int, 0>{}, t0);
-      if (t0 + C < t_end) step(std::integral_constant<int, 1>{}, t0 + C);
+    for (int t0 = t_beg; t0 < t_end; t0 += STAGES * C) {
+      sdpa::static_for<STAGES>([&](auto stage) {
+        constexpr int i = decltype(stage)::value;
+        if (i == 0 || t0 + i * C < t_end) step(stage, t0 + i * C);
+      });
     }
   }
 
@@ -724,12 +733,22 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
+  constexpr int STAGE = 3 * Tile<T, D>::BYTES;
   const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), block(D * 2);
   if (p.n_seg > 1) {
     hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, block, 0, st, p);
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
   }
-  hipLaunchKernelGGL((linear_attn_kernel<T, D>), grid, block, 0, st, p);
+  // A third chunk in flight helps where workgroups of the backward end up alone on their compute unit (D 128 bf16 backward:
+  // B8 S2048 H32 366 -> 334 us, B8 S4096 H32 727 -> 663; B4 S2048 H32 161 -> 164) and costs a little elsewhere (forward B1 S32768
+  // H32 359 -> 364, B8 S4096 H32 249 -> 252).
+  if (n_problems > 1 && p.n_seg == 1) {
+    auto kernel = linear_attn_kernel<T, D, 3>;
+    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 3 * STAGE)) return rc;
+    hipLaunchKernelGGL(kernel, grid, block, 3 * STAGE, st, p);
+  } else {
+    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), grid, block, 2 * STAGE, st, p);
+  }
   return status_from_hip(hipGetLastError());
 }
 
