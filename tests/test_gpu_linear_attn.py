@@ -447,10 +447,10 @@ def test_refusals(device):
     g = decays(2, device)
     with pytest.raises(ValueError):
         _ops().linear_attn(q, q, q, g.cpu(), None, None, 1.0)  # another device
-    with pytest.raises(_xops()._lib.XgError):
+    with pytest.raises(RuntimeError, match="xg_linear_attn"):
         _ops().linear_attn(q, q, q, g, None, None, math.nan)
     t = q[:, :, :1]
-    with pytest.raises(_xops()._lib.XgError):  # one state seen twice
+    with pytest.raises(RuntimeError, match="xg_linear_attn"):  # one state seen twice
         _ops().linear_attn_step(t, t, t, g, torch.zeros(1, 1, 64, 64, device=device).expand(1, 2, 64, 64), 1.0)
     with pytest.raises(ValueError):  # a state that could not be updated in place
         _ops().linear_attn_step(t, t, t, g, torch.zeros(1, 2, 64, 64, device=device).transpose(2, 3), 1.0)

@@ -8,7 +8,7 @@ each of at most the magnitude of the terms that are added."""
 import pytest
 import torch
 
-from xpu_graph_amd import HIPGraphRunner, _lib
+from xpu_graph_amd import HIPGraphRunner
 
 pytestmark = pytest.mark.gpu
 
@@ -388,4 +388,3 @@ def test_the_kernels_refuse_what_they_cannot_take(device):
         _ops().rope_axes(x, cos, sin, torch.zeros(4, dtype=torch.int64), [])  # positions on the host
     with pytest.raises(ValueError):
         _ops().qk_norm_rope(x, x[..., :32], None, None, cos, sin, None, [], False, 1e-6)
-    assert issubclass(_lib.XgError, RuntimeError)

@@ -6,20 +6,13 @@ import pytest
 import torch
 
 from xpu_graph_amd import _lib
-from xpu_graph_amd import ops as xops
+from xpu_graph_amd import ops as xops  # noqa: F401
 
 OPS = torch.ops.xpu_ops
 
 
 def meta(*shape, dtype=torch.bfloat16):
     return torch.empty(shape, dtype=dtype, device="meta")
-
-
-def test_axis_maps():
-    assert xops.rope_pair_axes((2, 3, 1)) == bytes([0, 0, 1, 1, 1, 2])
-    assert xops.rope_pair_axes((4, 2, 2), True) == bytes([0, 1, 2, 0, 1, 2, 0, 0])
-    assert xops.rope_pair_axes((8,), True) == bytes(8)
-    assert xops.rope_pair_axes((0, 3, 5), True) == bytes([0, 1, 2, 0, 1, 2, 0, 1])
 
 
 @pytest.mark.parametrize(

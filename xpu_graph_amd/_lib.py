@@ -10,6 +10,7 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libxpu_graph_amd.so")
+TORCH_OPS_PATH = os.path.join(_HERE, "libxpu_graph_amd_torch.so")  # csrc/torch_ops.cpp, on top of the kernel library
 
 # xg_dtype / xg_act values of include/xpu_graph_amd.h
 XG_F32, XG_F16, XG_BF16, XG_FP8_E4M3 = 0, 1, 2, 3
@@ -195,6 +196,10 @@ def exported_symbols():
 
 def is_built():
     return os.path.exists(LIB_PATH)
+
+
+def torch_ops_built():
+    return is_built() and os.path.exists(TORCH_OPS_PATH)
 
 
 def lib():

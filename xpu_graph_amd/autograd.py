@@ -15,11 +15,6 @@ a few microseconds of dispatch, which inference-only processes should not pay.
     dense(x, W, trans, bias, residual, act)   y = act(x W(^T) + bias + residual)
     dense_glu(x, Wg, Wu)       y = silu(x Wg^T) * (x Wu^T)
     rope(x, cos, sin)          y = x * cos + rotate_half(x) * sin,  rotate_half(x) = cat(-x[D/2:], x[:D/2])
-    rope_axes(x, cos, sin, positions, ...)   the rotation with gathered positions (gradient: the transposed rotation)
-    qk_norm_rope(q, k, wq, wk, cos, sin, positions, ..., eps)   rotation of the per-head RMS norms of q and k (gradients: the fused
-                               xg_qk_norm_rope_bwd kernel; the tables of both ops get none)
-    linear_attn(q, k, v, log_decay, state, lengths, scale)   y_t = scale q_t S_t, S_t = exp(log_decay) S_{t-1} + k_t v_t^T (gradients: the
-                               same kernel with the operands in other roles, xg_linear_attn_bwd; log_decay gets none)
     sdpa(q, k, v, causal, scale)   y = softmax(scale q k^T [+ causal mask]) v
     sdpa_lse(q, k, v, causal, scale)   the same, also returning the log-sum-exp of every row for the backward kernels
     sdpa_masked(q, k, v, mask, scale_t, causal, scale) / sdpa_masked_lse   with an additive mask and / or the scale in a
@@ -33,6 +28,9 @@ takes in place through xpu_ops::dense_at (shapes it does not take -- a dimension
 an Aten matmul).  For activations whose derivative cannot be told from the output (silu, gelu) the pre-activation is
 recomputed with one more dense call.  The gated layer saves only its inputs: both projections are recomputed on the
 dense kernel, the two input-gradient products run as one chain (the second takes the first as its residual).
+
+rope_axes, qk_norm_rope and linear_attn have their formulas beside their implementations in csrc/torch_ops.cpp, always
+registered: in C++ they cost an inference call nothing that could be measured.
 """
 import torch
 
@@ -283,107 +281,6 @@ def _rope_backward(ctx, gy):
     return gx, gcos, gsin
 
 
-# The three ops below go through torch.autograd.Function at the Autograd dispatch key instead of register_autograd: the
-# bookkeeping of the latter (defaults, metadata and pytrees of every call) costs 15 to 30 us a call, more than their kernels take
-# at small sizes.  Tracers see the same: the op itself in the forward graph, its *_bwd op in the backward graph.
-_PLAIN = (torch.Tensor, torch.nn.Parameter)
-
-
-def _below_autograd(name, first, *args):
-    """The op without its autograd formula.  Plain GPU tensors go straight to what the dispatcher would call."""
-    if first.__class__ in _PLAIN and first.is_cuda and not torch._C._len_torch_dispatch_stack() and torch._C._functorch.peek_interpreter_stack() is None:
-        from . import ops
-
-        return getattr(ops, "_" + name)(first, *args)
-    with torch._C._AutoDispatchBelowAutograd():
-        return getattr(torch.ops.xpu_ops, name).default(first, *args)
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-class _RopeAxes(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, cos, sin, positions, sections, interleaved):
-        ctx.sections, ctx.interleaved = sections, interleaved
-        ctx.save_for_backward(cos, sin, positions)
-        return _below_autograd("rope_axes", x, cos, sin, positions, sections, interleaved)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy):
-        return _below_autograd("rope_axes_bwd", gy, *ctx.saved_tensors, ctx.sections, ctx.interleaved), None, None, None, None, None
-
-
-def _rope_axes(x, cos, sin, positions, sections, interleaved=False):
-    if _wants_grad(cos, sin):
-        raise NotImplementedError("xpu_ops::rope_axes: no gradient for the cos / sin tables")
-    if _wants_grad(x):
-        return _RopeAxes.apply(x, cos, sin, positions, sections, interleaved)
-    return _below_autograd("rope_axes", x, cos, sin, positions, sections, interleaved)
-
-
-class _QkNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm):
-        ctx.sections, ctx.interleaved, ctx.eps = sections, interleaved, eps
-        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
-        return _below_autograd("qk_norm_rope", q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gq, gk):
-        q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, gwq, gwk = _below_autograd("qk_norm_rope_bwd", q, k, wq, wk, gq, gk, cos, sin, positions, ctx.sections, ctx.interleaved, ctx.eps,
-                                           need[2] or need[3])
-        return dq, dk, gwq if need[2] else None, gwk if need[3] else None, None, None, None, None, None, None, None
-
-
-def _qk_norm_rope(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm=False):
-    if _wants_grad(cos, sin):
-        raise NotImplementedError("xpu_ops::qk_norm_rope: no gradient for the cos / sin tables")
-    if _wants_grad(q, k, wq, wk):
-        return _QkNormRope.apply(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
-    return _below_autograd("qk_norm_rope", q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm)
-
-
-class _LinearAttn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, log_decay, state, lengths, scale):
-        ctx.scale = scale
-        ctx.save_for_backward(q, k, v, log_decay, state, lengths)
-        ctx.set_materialize_grads(False)  # an unused output hands over None: no gradient of the final state is read then
-        return _below_autograd("linear_attn", q, k, v, log_decay, state, lengths, scale)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, g_state):
-        if gy is None and g_state is None:
-            return None, None, None, None, None, None, None
-        q, k, v, log_decay, state, lengths = ctx.saved_tensors
-        if gy is None:
-            gy = torch.zeros_like(q)
-        want = ctx.needs_input_grad[4]
-        dq, dk, dv, d_state = _below_autograd("linear_attn_bwd", q, k, v, log_decay, state, lengths, gy, g_state, ctx.scale, want)
-        return dq, dk, dv, None, d_state if want else None, None, None
-
-
-def _linear_attn(q, k, v, log_decay, state, lengths, scale):
-    if _wants_grad(log_decay):
-        raise NotImplementedError("xpu_ops::linear_attn: no gradient for log_decay (only q, k, v and the state are differentiable)")
-    if _wants_grad(q, k, v, state):
-        return _LinearAttn.apply(q, k, v, log_decay, state, lengths, scale)
-    return _below_autograd("linear_attn", q, k, v, log_decay, state, lengths, scale)
-
-
-def _linear_attn_step(q, k, v, log_decay, state, scale):
-    if _wants_grad(q, k, v, log_decay, state):
-        raise NotImplementedError("xpu_ops::linear_attn_step: no gradient (the state is updated in place; use linear_attn to train)")
-    return _below_autograd("linear_attn_step", q, k, v, log_decay, state, scale)
-
-
 def _sdpa_setup(ctx, inputs, output):
     q, k, v, ctx.causal, ctx.scale = inputs
     ctx.save_for_backward(q, k, v)
@@ -526,10 +423,6 @@ def register():
     reg("xpu_ops::dense_glu", _dense_glu_backward, setup_context=_dense_glu_setup)
     reg("xpu_ops::dense_glu_save", _dense_glu_save_backward, setup_context=_dense_glu_save_setup)
     reg("xpu_ops::rope", _rope_backward, setup_context=_rope_setup)
-    from . import ops
-
-    for name, fn in (("rope_axes", _rope_axes), ("qk_norm_rope", _qk_norm_rope), ("linear_attn", _linear_attn), ("linear_attn_step", _linear_attn_step)):
-        ops._library.impl(name, fn, "Autograd")
     reg("xpu_ops::sdpa", _sdpa_backward, setup_context=_sdpa_setup)
     reg("xpu_ops::sdpa_lse", _sdpa_lse_backward, setup_context=_sdpa_lse_setup)
     reg("xpu_ops::sdpa_masked", _sdpa_masked_backward, setup_context=_sdpa_masked_setup)
@@ -540,7 +433,7 @@ def register():
         reg(f"xpu_ops::{op}", backward, setup_context=setup)
     # An op that was traced before (an inference compile earlier in the process) has its dispatch decisions cached
     # on the Python side; a stale entry for the Autograd key would keep sending traces to the "no formula" fallback.
-    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "rope_axes", "qk_norm_rope", "linear_attn", "linear_attn_step", "sdpa", "sdpa_lse",
+    for name in ("rms_norm", "layer_norm", "silu_mul2", "silu_mul", "act", "dense", "dense_glu", "dense_glu_save", "rope", "sdpa", "sdpa_lse",
                  "sdpa_masked", "sdpa_masked_lse", "add_rms_norm", "add_rms_norm_only", "add_layer_norm", "add_layer_norm_only"):
         packet = getattr(torch.ops.xpu_ops, name)
         for overload in packet.overloads():

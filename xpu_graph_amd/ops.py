@@ -3,7 +3,9 @@
 Each op has a schema, a Meta (fake-tensor) implementation so that the pass
 pipeline can re-propagate shapes through rewritten graphs, and ONE real
 implementation, registered for the CUDA dispatch key (HIP on ROCm), that hands
-raw device pointers and the current stream to the C-ABI kernel library.  There
+raw device pointers and the current stream to the C-ABI kernel library (in
+Python here; for the ops of an attention layer whose calls are bound by the
+host, in csrc/torch_ops.cpp).  There
 is deliberately no CPU implementation: calling an op on CPU tensors raises
 NotImplementedError from the dispatcher.
 
@@ -11,7 +13,6 @@ Op names follow the reference's convention of a vendor op namespace allowed
 inside device graphs (`xpu_ops`, src/xpu_graph/backends/device_graph.py:26-29).
 """
 import ctypes
-import functools
 from typing import List, Optional
 
 import torch
@@ -1225,6 +1226,16 @@ _library.impl("rope", _rope_meta, "Meta")
 
 
 # ------------------------------------------------ query / key preparation
+# Schemas and Meta implementations; what runs on the GPU, and the gradients, are in csrc/torch_ops.cpp (loaded below).
+#
+# rope_axes: rotary positions with several axes.  Pair i < R/2 of a row, (x[i], x[i + R/2]) with R = 2 * sum(sections), turns by row
+#   positions[axis of i, b, s] of the tables; columns from R on pass through.  The axes own runs of pairs, sections[0] of them
+#   axis 0's and so on; interleaved: pair i belongs to axis i % n while i < n * sections[i % n], and to axis 0 from there on.
+#   Without sections: one axis, R = D.  cos / sin: [P, R/2] (a column per pair) or [P, R] (one per element).  positions:
+#   [axes, B, S] (one axis: also [B, S], [S]; None: row s, or the only row).  A position outside the tables gives NaN.
+# qk_norm_rope: RMS norm over each head of q and of k, then that rotation, in one launch for both.  round_norm rounds the
+#   normalised rows to the tensors' dtype before they turn, as rms_norm followed by rope does.
+# rope_axes_bwd, qk_norm_rope_bwd: their gradients (of x; of q, k and the weights, empty where not wanted).
 _library.define("rope_axes(Tensor x, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
 _library.define("rope_axes_bwd(Tensor gy, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
 _library.define(
@@ -1239,285 +1250,89 @@ _library.define(
 ROPE_MAX_AXES = 4
 ROPE_MAX_HEAD_DIM = 512
 
-# What a call needs besides its pointers follows from shapes, strides and types alone; it is worked out once for each of them
-# (the small caches below) because a decode step would otherwise spend most of its time on it.
-
-
-def _same_device(first, *others):
-    index = first.get_device()
-    for t in others:
-        if t is not None and t.get_device() != index:
-            raise ValueError(f"xpu_ops: tensors on different devices ({first.device} and {t.device})")
-
-
-def _call(device, fn, what, *args):
-    """One launch on the current stream of the device of index `device`, whatever the current device is."""
-    if device == _current_device():
-        status = fn(*args, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            status = fn(*args, _raw_stream(device))
-    if status:
-        _lib.check(status, what)
-
-
-def _contiguous_strides(shape):
-    strides, step = [], 1
-    for n in reversed(shape):
-        strides.append(step)
-        step *= max(n, 1)
-    return tuple(reversed(strides))
-
-
-@functools.lru_cache(maxsize=4096)
-def _c_strides(strides, n=3):
-    """The first n element strides as the C entry points take them (they only read them)."""
-    return (ctypes.c_int64 * n)(*strides[:n])
-
-
-@functools.lru_cache(maxsize=4096)
-def _layout(shape, strides, per16):
-    """(whether the kernels can read it in place, the strides of a result in its layout): see _unit_last and
-    _empty_like_layout.  An unaligned start changes neither: such a tensor is copied in its own layout."""
-    if strides[-1] == 1 and all(st % per16 == 0 for st in strides[:-1]):
-        expect = 1
-        for st, n in sorted((st, n) for st, n in zip(strides, shape) if n != 1):
-            if st != expect:
-                return True, _contiguous_strides(shape)
-            expect *= n
-        return True, strides
-    return False, _contiguous_strides(shape)
-
-
-def _operand(t):
-    """(the tensor, or a copy that the kernels can read, the strides of a result in its layout)."""
-    in_place, strides = _layout(t.shape, t.stride(), 16 // t.element_size())
-    if not in_place:
-        t = t.contiguous()
-    if t.data_ptr() % 16:
-        t = t.clone()
-    return t, strides
-
-
-def _result(t, strides):
-    return torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
-
 
 def _result_meta(t):
-    """What _result allocates, from sizes that may be symbolic."""
+    """A result in the layout of t where the kernels read that in place and it is dense, else contiguous.  (The real ops copy an
+    unaligned tensor in its own layout, so alignment does not change it.)"""
     per16 = 16 // t.element_size()
     if t.stride(-1) == 1 and all(st % per16 == 0 for st in t.stride()[:-1]):
         return _empty_like_layout(t)
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-@functools.lru_cache(maxsize=256)
-def rope_pair_axes(sections, interleaved=False):
-    """The axis that turns each of the sum(sections) pairs of a row, as bytes.  In runs: the first sections[0] pairs belong
-    to axis 0, the next sections[1] to axis 1, ...; interleaved: pair i belongs to axis i % n while i < n * sections[i % n],
-    and to axis 0 from there on."""
-    n = len(sections)
-    if not interleaved:
-        return bytes(a for a, count in enumerate(sections) for _ in range(count))
-    return bytes(i % n if i < n * sections[i % n] else 0 for i in range(sum(sections)))
-
-
-def _rotary_check(x_shape, x_dtype, cos_shape, sin_shape, cos_dtype, sin_dtype, pos_shape, pos_dtype, sections):
-    """Refuses what the rotation cannot take; returns (rotated columns, table columns, axes)."""
-    if len(x_shape) != 4:
+def _rotary_check(x, cos, sin, positions, sections):
+    """Refuses what the rotation cannot take."""
+    _code(x.dtype)
+    if x.dim() != 4:
         raise ValueError("rope_axes: q, k or x must be [B, H, S, D]")
-    B, _, S, D = x_shape
+    B, _, S, D = x.shape
     if D % 16 != 0 or not 0 < D <= ROPE_MAX_HEAD_DIM:
         raise ValueError(f"rope_axes: head dim must be a multiple of 16, at most {ROPE_MAX_HEAD_DIM}")
-    if cos_shape != sin_shape or len(cos_shape) < 1 or any(d != 1 for d in cos_shape[:-2]):
+    if cos.shape != sin.shape or cos.dim() < 1 or any(d != 1 for d in cos.shape[:-2]):
         raise ValueError("rope_axes: cos / sin must be [P, R] or [P, R/2] tables of one shape (leading dims of size 1 allowed)")
-    if cos_dtype != sin_dtype or cos_dtype not in (x_dtype, torch.float32):
+    if cos.dtype != sin.dtype or cos.dtype not in (x.dtype, torch.float32):
         raise TypeError("rope_axes: cos / sin must share a dtype, that of x or float32")
-    cols = cos_shape[-1]
     axes = len(sections) or 1
     if axes > ROPE_MAX_AXES or any(n < 0 for n in sections):
         raise ValueError(f"rope_axes: sections are the pairs of each axis, at most {ROPE_MAX_AXES} axes")
     rot = 2 * sum(sections) if sections else D
-    if rot <= 0 or rot > D or rot % 16 != 0 or cols not in (rot, rot // 2):
+    if rot <= 0 or rot > D or rot % 16 != 0 or cos.shape[-1] not in (rot, rot // 2):
         raise ValueError("rope_axes: 2 * sum(sections) = R must be a multiple of 16 up to the head dim, the tables R or R/2 columns wide")
-    rows = cos_shape[-2] if len(cos_shape) > 1 else 1
-    if pos_shape is None:
+    rows = cos.shape[-2] if cos.dim() > 1 else 1
+    if positions is None:
         if axes != 1 or (rows != S and rows != 1):
             raise ValueError("rope_axes: without positions there is one axis and the tables have one row per token, or one row")
-    else:
-        if pos_dtype not in (torch.int32, torch.int64):
-            raise TypeError("rope_axes: positions must be int32 or int64")
-        full = (1,) * (3 - len(pos_shape)) + tuple(pos_shape)
-        if len(pos_shape) not in ((1, 2, 3) if axes == 1 else (3,)) or full[0] != axes or full[1] not in (1, B) or full[2] != S:
-            raise ValueError("rope_axes: positions must be [axes, B, S] ([S] or [B, S] with one axis; a batch dim of 1 is shared)")
-        if rows == 0:
-            raise ValueError("rope_axes: the tables are empty")
-    return rot, cols, axes
-
-
-def _rotary_check_tensors(x, cos, sin, positions, sections):
-    pos = (None, None) if positions is None else (positions.shape, positions.dtype)
-    return _rotary_check(x.shape, x.dtype, cos.shape, sin.shape, cos.dtype, sin.dtype, *pos, sections)
-
-
-@functools.lru_cache(maxsize=1024)
-def _rotary_plan(x_shape, x_dtype, cos_shape, cos_strides, cos_dtype, sin_shape, sin_strides, sin_dtype, pos_shape, pos_strides, pos_dtype,
-                 sections, interleaved):
-    """(an xg_rotary without pointers, what its axis map lives in, whether the tables can be read in place)."""
-    rot, cols, axes = _rotary_check(x_shape, x_dtype, cos_shape, sin_shape, cos_dtype, sin_dtype, pos_shape, pos_dtype, sections)
-    r = _lib.XgRotary(None, None, cos_shape[-2] if len(cos_shape) > 1 else 1, cols, cols, rot)
-    r.table_dtype, r.axes = _code(cos_dtype), axes
-    per16 = 16 // torch.empty((), dtype=cos_dtype).element_size()
-    in_place = len(cos_shape) > 1 and cos_strides == sin_strides and cos_strides[-1] == 1 and cos_strides[-2] >= cols and cos_strides[-2] % per16 == 0
-    if in_place:
-        r.table_stride = cos_strides[-2]
-    if pos_shape is not None:
-        r.positions_64bit = int(pos_dtype == torch.int64)
-        strides = (0,) * (3 - len(pos_shape)) + pos_strides
-        r.pos_strides[0], r.pos_strides[2] = strides[0], strides[2]
-        r.pos_strides[1] = strides[1] if len(pos_shape) > 1 and pos_shape[-2] > 1 else 0
-    pair_axis = rope_pair_axes(sections, interleaved) if axes > 1 else None
-    r.pair_axis = pair_axis
-    return r, pair_axis, in_place
-
-
-def _rotary(x, cos, sin, positions, sections, interleaved):
-    """The xg_rotary of a call and the tables it points to."""
-    pos = (None, None, None) if positions is None else (positions.shape, positions.stride(), positions.dtype)
-    plan, _, in_place = _rotary_plan(x.shape, x.dtype, cos.shape, cos.stride(), cos.dtype, sin.shape, sin.stride(), sin.dtype, *pos, tuple(sections),
-                                     bool(interleaved))
-    _same_device(x, cos, sin, positions)
-    c, s = cos.data_ptr(), sin.data_ptr()
-    if not in_place or c % 16 or s % 16:
-        cos, sin = (t.reshape(-1, t.shape[-1]).clone(memory_format=torch.contiguous_format) for t in (cos, sin))
-        c, s = cos.data_ptr(), sin.data_ptr()
-    r = _lib.XgRotary.from_buffer_copy(plan)
-    if not in_place or r.table_stride != cos.stride(-2):
-        r.table_stride = cos.shape[-1]
-    r.cos_table, r.sin_table = c, s
-    if positions is not None:
-        r.positions = positions.data_ptr()
-    return r, (cos, sin)
-
-
-def _rope_axes_run(x, cos, sin, positions, sections, interleaved, transpose):
-    code = _code(x.dtype)
-    r, _keep = _rotary(x, cos, sin, positions, sections, interleaved)
-    x, strides = _operand(x)
-    out = _result(x, strides)
-    B, H, S, D = x.shape
-    if B and H and S:
-        _call(x.get_device(), _lib.lib().xg_rope_axes, "xg_rope_axes", x.data_ptr(), out.data_ptr(), B, H, S, D, _c_strides(x.stride()),
-              _c_strides(strides), r, transpose, code)
-    return out
-
-
-def _rope_axes(x, cos, sin, positions, sections, interleaved=False):
-    """Rotary positions with several axes: pair i of a row turns by row positions[axis of i, b, s] of the tables (see
-    rope_pair_axes); columns from R = 2 * sum(sections) on pass through.  Without sections: one axis, R = D."""
-    return _rope_axes_run(x, cos, sin, positions, sections, interleaved, 0)
-
-
-def _rope_axes_bwd(gy, cos, sin, positions, sections, interleaved=False):
-    """The gradient of x: the transposed rotation of gy."""
-    return _rope_axes_run(gy, cos, sin, positions, sections, interleaved, 1)
+        return
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError("rope_axes: positions must be int32 or int64")
+    shape = tuple(positions.shape)
+    full = (1,) * (3 - len(shape)) + shape
+    if len(shape) not in ((1, 2, 3) if axes == 1 else (3,)) or full[0] != axes or full[1] not in (1, B) or full[2] != S:
+        raise ValueError("rope_axes: positions must be [axes, B, S] ([S] or [B, S] with one axis; a batch dim of 1 is shared)")
+    if rows == 0:
+        raise ValueError("rope_axes: the tables are empty")
 
 
 def _rope_axes_meta(x, cos, sin, positions, sections, interleaved=False):
-    _rotary_check_tensors(x, cos, sin, positions, sections)
+    _rotary_check(x, cos, sin, positions, sections)
     return _result_meta(x)
 
 
 def _qk_check(q, k, q_weight, k_weight):
-    qs, ks = q.shape, k.shape
-    if len(qs) != 4 or len(ks) != 4 or qs[0] != ks[0] or qs[2:] != ks[2:]:
+    if q.dim() != 4 or k.dim() != 4 or q.shape[0] != k.shape[0] or q.shape[2:] != k.shape[2:]:
         raise ValueError("qk_norm_rope: q and k must be [B, H, S, D] and [B, Hkv, S, D]")
     if q.dtype != k.dtype:
         raise TypeError("qk_norm_rope: q and k must share a dtype")
     for w in (q_weight, k_weight):
-        if w is not None and (w.dim() != 1 or w.shape[0] != qs[3]):
+        if w is not None and (w.dim() != 1 or w.shape[0] != q.shape[3]):
             raise ValueError("qk_norm_rope: a weight is one row of the head dim")
-
-
-def _qk_weights(q, q_weight, k_weight):
-    (q_weight, k_weight), w_dtype = _param_dtype(q.dtype, q_weight, k_weight)
-    # the kernel reads 16 bytes at a time; a weight that is a slice of a larger tensor may start anywhere
-    q_weight, k_weight = (w.clone() if w is not None and w.data_ptr() % 16 else w for w in (q_weight, k_weight))
-    return q_weight, k_weight, w_dtype
-
-
-def _qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps, round_norm=False):
-    """RMS norm over each head of q and of k and the rotation of rope_axes, in one launch for both.  round_norm rounds the
-    normalised rows to the tensors' dtype before they turn, as rms_norm followed by rope does."""
-    _qk_check(q, k, q_weight, k_weight)
-    code = _code(q.dtype)
-    _same_device(q, k, q_weight, k_weight)
-    r, _keep = _rotary(q, cos, sin, positions, sections, interleaved)
-    (q, qo_strides), (k, ko_strides) = _operand(q), _operand(k)
-    q_out, k_out = _result(q, qo_strides), _result(k, ko_strides)
-    B, H, S, D = q.shape
-    Hkv = k.shape[1]
-    if B and S and (H or Hkv):
-        q_weight, k_weight, w_dtype = _qk_weights(q, q_weight, k_weight)
-        _call(q.get_device(), _lib.lib().xg_qk_norm_rope, "xg_qk_norm_rope", q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight),
-              q_out.data_ptr(), k_out.data_ptr(), B, H, Hkv, S, D, _c_strides(q.stride()), _c_strides(k.stride()), _c_strides(qo_strides),
-              _c_strides(ko_strides), r, eps, 1 if round_norm else 0, code, _code(w_dtype))
-    return q_out, k_out
 
 
 def _qk_norm_rope_meta(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps, round_norm=False):
     _qk_check(q, k, q_weight, k_weight)
-    _rotary_check_tensors(q, cos, sin, positions, sections)
+    _rotary_check(q, cos, sin, positions, sections)
     return _result_meta(q), _result_meta(k)
-
-
-def _qk_norm_rope_bwd(q, k, q_weight, k_weight, gq, gk, cos, sin, positions, sections, interleaved, eps, want_gw):
-    """(dq, dk, gw_q, gw_k) for the upstream gradients of the two outputs; the weight gradients are empty when not wanted
-    or without a weight."""
-    _qk_check(q, k, q_weight, k_weight)
-    if gq.shape != q.shape or gk.shape != k.shape or gq.dtype != q.dtype or gk.dtype != q.dtype:
-        raise ValueError("qk_norm_rope_bwd: gq and gk must match q and k in shape and dtype")
-    code = _code(q.dtype)
-    _same_device(q, k, q_weight, k_weight, gq, gk)
-    r, _keep = _rotary(q, cos, sin, positions, sections, interleaved)
-    (q, dq_strides), (k, dk_strides), (gq, _), (gk, _) = _operand(q), _operand(k), _operand(gq), _operand(gk)
-    dq, dk = _result(q, dq_strides), _result(k, dk_strides)
-    gws = [torch.empty(w.shape, dtype=w.dtype, device=q.device) if want_gw and w is not None else None for w in (q_weight, k_weight)]
-    B, H, S, D = q.shape
-    Hkv = k.shape[1]
-    if not (B and S and (H or Hkv)):
-        gws = [g.zero_() if g is not None else None for g in gws]
-    else:
-        wq, wk, w_dtype = _qk_weights(q, q_weight, k_weight)
-        kernel_gws = [torch.empty_like(g, dtype=w_dtype) if g is not None and g.dtype != w_dtype else g for g in gws]
-        lib = _lib.lib()
-        n_ws = lib.xg_qk_norm_rope_bwd_workspace_floats(B, H, Hkv, S, D) if want_gw else 0
-        ws = _workspace(n_ws, q.device)
-        _call(q.get_device(), lib.xg_qk_norm_rope_bwd, "xg_qk_norm_rope_bwd", q.data_ptr(), k.data_ptr(), _ptr(wq), _ptr(wk), gq.data_ptr(),
-              gk.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(kernel_gws[0]), _ptr(kernel_gws[1]), _ptr(ws), n_ws, B, H, Hkv, S, D,
-              *(_c_strides(t.stride()) for t in (q, k, gq, gk)), _c_strides(dq_strides), _c_strides(dk_strides), r, eps, code, _code(w_dtype))
-        gws = [a if a is b else a.copy_(b) for a, b in zip(gws, kernel_gws)]
-    return dq, dk, *(torch.empty(0, dtype=q.dtype, device=q.device) if g is None else g for g in gws)
 
 
 def _qk_norm_rope_bwd_meta(q, k, q_weight, k_weight, gq, gk, cos, sin, positions, sections, interleaved, eps, want_gw):
     _qk_check(q, k, q_weight, k_weight)
-    none = lambda: torch.empty(0, dtype=q.dtype, device=q.device)  # noqa: E731
-    gws = [torch.empty(w.shape, dtype=w.dtype, device=q.device) if want_gw and w is not None else none() for w in (q_weight, k_weight)]
+    _rotary_check(q, cos, sin, positions, sections)
+    if gq.shape != q.shape or gk.shape != k.shape or gq.dtype != q.dtype or gk.dtype != q.dtype:
+        raise ValueError("qk_norm_rope_bwd: gq and gk must match q and k in shape, dtype and device")
+    gws = (
+        torch.empty((q.shape[3] if want_gw and w is not None else 0,), dtype=q.dtype if w is None else w.dtype, device=q.device)
+        for w in (q_weight, k_weight)
+    )
     return _result_meta(q), _result_meta(k), *gws
 
 
-_library.impl("rope_axes", _rope_axes, "CUDA")
-_library.impl("rope_axes", _rope_axes_meta, "Meta")
-_library.impl("rope_axes_bwd", _rope_axes_bwd, "CUDA")
-_library.impl("rope_axes_bwd", _rope_axes_meta, "Meta")
-_library.impl("qk_norm_rope", _qk_norm_rope, "CUDA")
-_library.impl("qk_norm_rope", _qk_norm_rope_meta, "Meta")
-_library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd, "CUDA")
-_library.impl("qk_norm_rope_bwd", _qk_norm_rope_bwd_meta, "Meta")
-
-
 # ------------------------------------------------------- linear attention
+# linear_attn: S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t over a sequence: (out, the state after each entry's last
+#   token).  state: the one before the first token (zeros without); lengths [B]: tokens from there on are not read, give zeros and
+#   do not reach the state.  q [B, H, S, D], k and v [B, Hkv, S, D], log_decay float32 [H], states float32 [B, H, D, D].
+# linear_attn_bwd: (dq, dk, dv, d_state) from the gradients of the two outputs (d_state_out may be None; d_state is empty when not
+#   wanted).  log_decay gets none.
+# linear_attn_step: one token; the state is updated in place, the output row comes out of the same pass.
 _library.define(
     "linear_attn(Tensor q, Tensor k, Tensor v, Tensor log_decay, Tensor? state, Tensor? lengths, float scale) -> (Tensor, Tensor)"
 )
@@ -1529,17 +1344,15 @@ _library.define("linear_attn_step(Tensor q, Tensor k, Tensor v, Tensor log_decay
 
 
 def _linear_attn_check(q, k, v, log_decay, state, lengths=None):
-    qs, ks = q.shape, k.shape
-    if len(qs) != 4 or len(ks) != 4 or ks != v.shape:
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
         raise ValueError("linear_attn: q must be [B, H, S, D], k and v [B, Hkv, S, D]")
-    B, H, S, D = qs
-    Hkv = ks[1]
-    if ks[0] != B or ks[2] != S or ks[3] != D or (H % Hkv != 0 if Hkv else H != 0):
+    B, H, S, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape[0] != B or k.shape[2] != S or k.shape[3] != D or (H % Hkv != 0 if Hkv else H != 0):
         raise ValueError("linear_attn: inconsistent q/k/v shapes")
     if D not in (64, 128):
         raise ValueError("linear_attn: head dim must be 64 or 128")
-    dtype = q.dtype
-    if (dtype != torch.bfloat16 and dtype != torch.float16) or k.dtype != dtype or v.dtype != dtype:
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
         raise TypeError("linear_attn: q, k, v must share a dtype, bfloat16 or float16")
     if log_decay.dim() != 1 or log_decay.shape[0] != H or log_decay.dtype != torch.float32:
         raise ValueError("linear_attn: log_decay must be float32 [H]")
@@ -1547,53 +1360,6 @@ def _linear_attn_check(q, k, v, log_decay, state, lengths=None):
         raise ValueError("linear_attn: states must be float32 [B, H, D, D]")
     if lengths is not None and (tuple(lengths.shape) != (B,) or lengths.dtype not in (torch.int32, torch.int64)):
         raise ValueError("linear_attn: lengths must be int32 or int64 [B]")
-    _same_device(q, k, v, log_decay, state, lengths)
-
-
-# Tokens further apart than this are copied together first: the kernels address a chunk of 32 rows by 32-bit offsets.
-_LINEAR_ATTN_MAX_PITCH = 1 << 26
-
-
-def _token_operand(t):
-    """_operand, with a distance between tokens that the chunked kernels take."""
-    t, strides = _operand(t)
-    return (t if t.stride(2) < _LINEAR_ATTN_MAX_PITCH else t.contiguous()), strides
-
-
-def _state_operand(state):
-    if state is None:
-        return None
-    state = state.contiguous()
-    return state.clone() if state.data_ptr() % 16 else state
-
-
-def _workspace(floats, device):
-    return torch.empty((floats,), dtype=torch.float32, device=device) if floats > 0 else None
-
-
-def _lengths_operand(lengths):
-    return (None, 0) if lengths is None else (lengths.contiguous(), int(lengths.dtype == torch.int64))
-
-
-def _linear_attn(q, k, v, log_decay, state, lengths, scale):
-    """S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t over a sequence: (out, the state after each entry's last
-    token).  state: the one before the first token (zeros without); lengths [B]: tokens from there on are not read, give zeros
-    and do not reach the state."""
-    _linear_attn_check(q, k, v, log_decay, state, lengths)
-    (q, o_strides), (k, _), (v, _) = _token_operand(q), _token_operand(k), _token_operand(v)
-    B, H, S, D = q.shape
-    out = _result(q, o_strides)
-    state_out = torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
-    if not (B and H and S):
-        return out, (state_out.zero_() if state is None else state_out.copy_(state))
-    state, log_decay, (lengths, wide) = _state_operand(state), log_decay.contiguous(), _lengths_operand(lengths)
-    lib = _lib.lib()
-    n_ws = lib.xg_linear_attn_workspace_floats(B, H, S, D)
-    ws = _workspace(n_ws, q.device)
-    _call(q.get_device(), lib.xg_linear_attn, "xg_linear_attn", q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(state),
-          _ptr(lengths), wide, out.data_ptr(), state_out.data_ptr(), _ptr(ws), n_ws, B, H, k.shape[1], S, D, _c_strides(q.stride()),
-          _c_strides(k.stride()), _c_strides(v.stride()), _c_strides(o_strides), scale, _code(q.dtype))
-    return out, state_out
 
 
 def _linear_attn_meta(q, k, v, log_decay, state, lengths, scale):
@@ -1602,83 +1368,53 @@ def _linear_attn_meta(q, k, v, log_decay, state, lengths, scale):
     return _result_meta(q), torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
 
 
-def _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out):
+def _linear_attn_bwd_meta(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
     _linear_attn_check(q, k, v, log_decay, state, lengths)
-    if d_out.shape != q.shape or d_out.dtype != q.dtype:
-        raise ValueError("linear_attn_bwd: d_out must match q in shape and dtype")
     B, H, _, D = q.shape
+    if d_out.shape != q.shape or d_out.dtype != q.dtype:
+        raise ValueError("linear_attn_bwd: d_out must match q in shape, dtype and device")
     if d_state_out is not None and (tuple(d_state_out.shape) != (B, H, D, D) or d_state_out.dtype != torch.float32):
         raise ValueError("linear_attn_bwd: d_state_out must be float32 [B, H, D, D]")
-    _same_device(q, d_out, d_state_out)
-
-
-def _linear_attn_bwd(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
-    """(dq, dk, dv, d_state): the gradients of linear_attn's inputs from those of its two outputs (d_state_out may be None);
-    d_state is empty when not wanted.  log_decay gets none."""
-    _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out)
-    (q, dq_strides), (k, dk_strides), (v, dv_strides), (d_out, _) = (_token_operand(t) for t in (q, k, v, d_out))
-    B, H, S, D = q.shape
-    dq, dk, dv = _result(q, dq_strides), _result(k, dk_strides), _result(v, dv_strides)
-    d_state = torch.empty((B, H, D, D) if want_d_state else (0,), dtype=torch.float32, device=q.device)
-    if not (B and H and S):
-        if want_d_state:
-            d_state.zero_() if d_state_out is None else d_state.copy_(d_state_out)
-        return dq, dk, dv, d_state
-    state, d_state_out, log_decay = _state_operand(state), _state_operand(d_state_out), log_decay.contiguous()
-    lengths, wide = _lengths_operand(lengths)
-    lib = _lib.lib()
-    Hkv = k.shape[1]
-    n_ws = lib.xg_linear_attn_bwd_workspace_floats(B, H, Hkv, S, D)
-    ws = _workspace(n_ws, q.device)
-    _call(q.get_device(), lib.xg_linear_attn_bwd, "xg_linear_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(state),
-          _ptr(lengths), wide, d_out.data_ptr(), _ptr(d_state_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-          d_state.data_ptr() if want_d_state else None, _ptr(ws), n_ws, B, H, Hkv, S, D, *(_c_strides(t.stride()) for t in (q, k, v, d_out)),
-          _c_strides(dq_strides), _c_strides(dk_strides), _c_strides(dv_strides), scale, _code(q.dtype))
-    return dq, dk, dv, d_state
-
-
-def _linear_attn_bwd_meta(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
-    _linear_attn_bwd_check(q, k, v, log_decay, state, lengths, d_out, d_state_out)
-    B, H, _, D = q.shape
     d_state = torch.empty((B, H, D, D) if want_d_state else (0,), dtype=torch.float32, device=q.device)
     return _result_meta(q), _result_meta(k), _result_meta(v), d_state
 
 
-def _linear_attn_step_check(q, k, v, log_decay, state):
+def _linear_attn_step_meta(q, k, v, log_decay, state, scale):
     _linear_attn_check(q, k, v, log_decay, state)
     if q.shape[2] != 1:
         raise ValueError("linear_attn_step: one token, q [B, H, 1, D]")
     if state.stride(3) != 1 or state.stride(2) != q.shape[3]:
         raise ValueError("linear_attn_step: the [D, D] matrices of the state must be contiguous (it is updated in place)")
-
-
-def _linear_attn_step(q, k, v, log_decay, state, scale):
-    """One token of linear_attn: the state is updated in place, the output row comes out of the same pass."""
-    _linear_attn_step_check(q, k, v, log_decay, state)
-    q, k, v = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k, v))
-    B, H, _, D = q.shape
-    out = torch.empty((B, H, 1, D), dtype=q.dtype, device=q.device)
-    if not (B and H):
-        return out
-    log_decay = log_decay.contiguous()
-    if not state.is_inference():
-        torch.autograd.graph.increment_version(state)  # a graph that saved the state must see that it changed
-    _call(q.get_device(), _lib.lib().xg_linear_attn_step, "xg_linear_attn_step", q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
-          state.data_ptr(), out.data_ptr(), B, H, k.shape[1], D, *(_c_strides(t.stride(), 2) for t in (q, k, v, out, state)), scale, _code(q.dtype))
-    return out
-
-
-def _linear_attn_step_meta(q, k, v, log_decay, state, scale):
-    _linear_attn_step_check(q, k, v, log_decay, state)
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 
-_library.impl("linear_attn", _linear_attn, "CUDA")
-_library.impl("linear_attn", _linear_attn_meta, "Meta")
-_library.impl("linear_attn_bwd", _linear_attn_bwd, "CUDA")
-_library.impl("linear_attn_bwd", _linear_attn_bwd_meta, "Meta")
-_library.impl("linear_attn_step", _linear_attn_step, "CUDA")
-_library.impl("linear_attn_step", _linear_attn_step_meta, "Meta")
+_NATIVE = {
+    "rope_axes": _rope_axes_meta,
+    "rope_axes_bwd": _rope_axes_meta,
+    "qk_norm_rope": _qk_norm_rope_meta,
+    "qk_norm_rope_bwd": _qk_norm_rope_bwd_meta,
+    "linear_attn": _linear_attn_meta,
+    "linear_attn_bwd": _linear_attn_bwd_meta,
+    "linear_attn_step": _linear_attn_step_meta,
+}
+for _name, _meta in _NATIVE.items():
+    _library.impl(_name, _meta, "Meta")
+
+
+def _load_native_ops():
+    """Their GPU implementations and gradients; without the library a call says how to build it."""
+    if _lib.torch_ops_built():
+        torch.ops.load_library(_lib.TORCH_OPS_PATH)
+        return
+
+    def missing(*args, **kwargs):
+        raise ImportError(f"{_lib.TORCH_OPS_PATH} is missing: the mi355x target has no fallback path. Build it with `python -m xpu_graph_amd.build`.")
+
+    for name in _NATIVE:
+        _library.impl(name, missing, "CUDA")
+
+
+_load_native_ops()
 
 
 # ------------------------------------------------------------- training
