@@ -457,13 +457,12 @@ int xg_rope(const void* x, const void* cos_table, const void* sin_table, void* o
  * x, q, k and their outputs are [B, heads, S, D] with element strides for
  * batch, head, sequence and a unit last stride; strides multiples of 16 bytes;
  * D % 16 == 0, D <= 512, R % 16 == 0, R <= D; dtype XG_BF16, XG_F16, XG_F32.
- * At most 2^31 - 1 rows (B S heads).
+ * At most 2^31 - 1 rows (B S heads) and 2^35 elements.
  *   xg_rope_axes: transpose != 0 applies the transposed rotation, which is the
  *     gradient of x.
  *   xg_qk_norm_rope: q [B,H,S,D] and k [B,Hkv,S,D] in one launch; either may
- *     have no heads.  round_norm != 0 rounds n to `dtype` before the rotation,
- *     as xg_rms_norm followed by xg_rope does (bit for bit in bf16 at D 64 and
- *     128, where the kernels add a row up in the same order).
+ *     have no heads.  n stays fp32 up to the rotation: each output is rounded
+ *     once, where xg_rms_norm followed by xg_rope rounds twice.
  *   xg_qk_norm_rope_bwd: dq, dk from the upstream gradients gq, gk of the two
  *     outputs, and gw_q, gw_k [D] (in w_dtype; NULL: not wanted), summed over
  *     rows in a fixed order (no atomics) through a workspace of
@@ -492,7 +491,7 @@ int xg_rope_axes(const void* x, void* out, int64_t B, int64_t H, int64_t S, int6
 int xg_qk_norm_rope(const void* q, const void* k, const void* q_w, const void* k_w, void* q_out, void* k_out, int64_t B,
                     int64_t H, int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3], const int64_t k_strides[3],
                     const int64_t qo_strides[3], const int64_t ko_strides[3], const xg_rotary* rotary, float eps,
-                    int round_norm, int dtype, int w_dtype, xg_stream_t stream);
+                    int dtype, int w_dtype, xg_stream_t stream);
 int64_t xg_qk_norm_rope_bwd_workspace_floats(int64_t B, int64_t H, int64_t Hkv, int64_t S, int64_t D);
 int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const void* k_w, const void* gq, const void* gk,
                         void* dq, void* dk, void* gw_q, void* gw_k, float* workspace, int64_t workspace_floats, int64_t B,
@@ -515,7 +514,8 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  *     [0, S]: tokens from there on are not read, do not reach the state, and
  *     give zeros in out and in the gradients.
  *   A NaN or an infinity in q, k or v reaches the outputs of its own chunk of
- *   32 tokens and of all later tokens.
+ *   32 tokens, before it too, and those of later tokens, at least while its
+ *   decayed weight is not zero in fp32.
  * xg_linear_attn: a whole sequence, 32 tokens at a time on the matrix cores.
  *   Up to three launches; workspace: xg_linear_attn_workspace_floats fp32 (0:
  *   none needed).

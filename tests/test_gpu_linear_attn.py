@@ -454,3 +454,93 @@ def test_refusals(device):
         _ops().linear_attn_step(t, t, t, g, torch.zeros(1, 1, 64, 64, device=device).expand(1, 2, 64, 64), 1.0)
     with pytest.raises(ValueError):  # a state that could not be updated in place
         _ops().linear_attn_step(t, t, t, g, torch.zeros(1, 2, 64, 64, device=device).transpose(2, 3), 1.0)
+
+def test_dimensions_of_one_element_have_no_stride_that_counts(device):
+    """Contiguous to torch, with strides of no whole 16 bytes where a dimension has one element."""
+    S, D = 70, 64
+    odd = lambda x: x.as_strided(x.shape, (x[0].numel() + 1, x[0, 0].numel() + 3, D, 1))  # noqa: E731
+    q, k, v, go = (odd(torch.randn(1, 1, S, D, device=device).bfloat16() * 0.3) for _ in range(4))
+    assert q.is_contiguous() and q.stride(0) % 8
+    g, s0 = decays(1, device), odd(torch.randn(1, 1, D, D, device=device))
+    run = lambda *a: (*_ops().linear_attn(*a[:3], g, a[4], None, 0.1), *_ops().linear_attn_bwd(*a[:3], g, a[4], None, a[3], a[4], 0.1, True))  # noqa: E731
+    args = (q, k, v, go, s0)
+    assert all(torch.equal(a, b) for a, b in zip(run(*args), run(*(x.reshape(-1).clone().view(x.shape) for x in args))))
+    t = (q[:, :, :1], k[:, :, :1], v[:, :, :1])
+    plain = s0.reshape(-1).clone().view(s0.shape)
+    st = odd(plain.clone())
+    assert torch.equal(_ops().linear_attn_step(*t, g, st, 0.1), _ops().linear_attn_step(*t, g, plain, 0.1)) and torch.equal(st, plain)
+    # one token, tokens of a huge pitch: nothing is copied or refused, nor is there a second token to reach
+    far = torch.as_strided(q.reshape(-1)[:D].clone(), (1, 1, 1, D), (1 << 40, 1 << 40, 1 << 40, 1))
+    assert torch.equal(_ops().linear_attn(far, far, far, g, None, None, 0.1)[0], _ops().linear_attn(*[q[:, :, :1]] * 3, g, None, None, 0.1)[0])
+
+
+def test_starts_off_16_bytes_are_copied(device):
+    B, H, S, D = 1, 2, 40, 64
+    args = [make((B, H, S, D), torch.bfloat16, device, i, "bhsd") for i in range(4)]
+    moved = []
+    for x in args:
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=device)[1:].view(x.shape)
+        moved.append(y.copy_(x))
+    g = decays(H, device)
+    s0 = torch.empty(B * H * D * D + 1, device=device)[1:].view(B, H, D, D).normal_()
+    run = lambda a, s: (*_ops().linear_attn(*a[:3], g, s, None, 0.1), *_ops().linear_attn_bwd(*a[:3], g, s, None, a[3], s, 0.1, True))  # noqa: E731
+    assert all(torch.equal(a, b) for a, b in zip(run(moved, s0), run(args, s0.clone())))
+    with pytest.raises(RuntimeError, match="xg_linear_attn_step"):  # a state is written where it lies
+        _ops().linear_attn_step(*(x[:, :, :1] for x in args[:3]), g, s0, 0.1)
+
+
+def test_a_training_pass_recorded_in_a_graph(device):
+    """Forward and backward through autograd in one recording, replayed on new values."""
+    B, H, S, D = 2, 2, 200, 64
+    g = decays(H, device)
+    static = [make((B, H, S, D), torch.bfloat16, device, i).requires_grad_() for i in range(3)]
+    s0, go = torch.randn(B, H, D, D, device=device).requires_grad_(), make((B, H, S, D), torch.bfloat16, device, 7)
+
+    def f():
+        o, s = _ops().linear_attn(*static, g, s0, None, 0.1)
+        grads = torch.autograd.grad((o, s), (*static, s0), (go, s.detach()))
+        return (o.detach(), s.detach(), *grads)  # (no graph of these leaves outlives a call)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        f()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = f()
+    for step in range(3):
+        with torch.no_grad():
+            for i, x in enumerate(static):
+                x.copy_(make((B, H, S, D), torch.bfloat16, device, 100 * (step + 1) + i))
+            s0.normal_()
+        graph.replay()
+        seen = [t.clone() for t in got]
+        assert all(torch.equal(a, b) for a, b in zip(f(), seen))
+
+
+def test_gradients_that_do_not_exist_are_refused(device):
+    g = decays(2, device)
+    q, k, v = (make((1, 2, 8, 64), torch.bfloat16, device, i).requires_grad_() for i in range(3))
+    o, _ = _ops().linear_attn(q, k, v, g, None, None, 0.1)
+    (dq,) = torch.autograd.grad(o, q, torch.ones_like(o).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="not implemented"):  # a gradient of a gradient
+        torch.autograd.grad(dq.sum(), k)
+    with pytest.raises(NotImplementedError, match="log_decay"):
+        _ops().linear_attn(q, k, v, g.clone().requires_grad_(), None, None, 0.1)
+    s0 = torch.zeros(1, 2, 64, 64, device=device)
+    with pytest.raises(NotImplementedError, match="linear_attn_step"):
+        _ops().linear_attn_step(q[:, :, :1], k[:, :, :1], v[:, :, :1], g, s0, 0.1)
+    with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        x = q.detach()
+        _ops().linear_attn(torch.autograd.forward_ad.make_dual(x, x), x, x, g, None, None, 0.1)
+    # a graph that needs the old state sees that a step has overwritten it
+    o, _ = _ops().linear_attn(q, k, v, g, s0, None, 0.1)
+    x = q.detach()[:, :, :1]
+    _ops().linear_attn_step(x, x, x, g, s0, 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    with torch.inference_mode():  # tensors without a version counter
+        s1 = torch.zeros(1, 2, 64, 64, device=device)
+        y = x.clone()
+        assert torch.equal(_ops().linear_attn_step(y, y, y, g, s1, 0.1), _ops().linear_attn_step(x, x, x, g, torch.zeros_like(s1), 0.1))

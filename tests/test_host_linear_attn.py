@@ -89,6 +89,7 @@ def test_entry_points_refuse_before_any_launch():
     assert fwd(q=None) == -4 and fwd(g=None) == -4 and fwd(out=None) == -4 and fwd(ws=None) == -4 and fwd(ws_n=need - 1) == -7
     assert fwd(q=off) == -3 and fwd(state=off) == -3 and fwd(qs=S3(1, 2, 3)) == -3 and fwd(qs=S3(-8, 8, 8)) == -2
     assert fwd(n=ctypes.c_void_p(p.value + 4)) == -3
+    assert fwd(qs=S3(1 << 14, 1 << 12, 1 << 26)) == -5  # tokens too far apart for 32-bit offsets within a chunk
     assert fwd(scale=float("nan")) == -7 and fwd(scale=float("inf")) == -7 and fwd(B=1 << 20, H=2) == -5
 
     need_b = lib.xg_linear_attn_bwd_workspace_floats(1, 2, 1, 1024, 64)

@@ -73,6 +73,22 @@ def test_layouts_survive():
     assert OPS.rope_axes(x, t, t, None, []).stride() == x.stride()
 
 
+def test_layouts_of_dimensions_of_one_element():
+    """What torch keeps as the stride of a dimension of size 1 does not decide about the layout."""
+    x = torch.empty(1, 3, 8, 64, device="meta", dtype=torch.bfloat16).as_strided((1, 3, 8, 64), (1 << 40, 64, 192, 1))
+    odd = torch.empty_strided((1, 3, 8, 64), (8 * 192 + 1, 64, 192, 1), device="meta", dtype=torch.bfloat16)
+    t = meta(8, 32, dtype=torch.float32)
+    for y in (x, odd):
+        assert OPS.rope_axes(y, t, t, None, []).stride()[1:] == (64, 192, 1)
+
+
+def test_the_gpu_implementations_are_built_and_loaded():
+    assert _lib.torch_ops_built()
+    for name in ("rope_axes", "rope_axes_bwd", "qk_norm_rope", "qk_norm_rope_bwd", "linear_attn", "linear_attn_bwd", "linear_attn_step"):
+        for key in ("CUDA", "Autograd", "Meta"):
+            assert torch._C._dispatch_has_kernel_for_dispatch_key(f"xpu_ops::{name}", key), (name, key)
+
+
 def test_cpu_tensors_have_no_kernel():
     x, t = torch.zeros(1, 1, 2, 64), torch.zeros(2, 32)
     with pytest.raises(NotImplementedError):
@@ -114,9 +130,10 @@ def test_entry_points_refuse_before_any_launch():
     assert rope(xs=S3(512, 250, 64)) == -3 and rope(xs=S3(512, -256, 64)) == -2 and rope(x=ctypes.c_void_p(p.value + 8)) == -3
     assert rope(table_stride=33) == -3 and rope(cos_table=p.value + 4) == -3 and rope(positions=p.value + 4) == -3
     assert rope(B=1 << 20, S=1 << 20) == -5  # more rows than a launch takes
+    assert rope(B=1 << 30, H=1, S=1, D=128) == -5  # more threads
 
     def qk(H=2, Hkv=1, w_dtype=2, k=p, r=None):
-        return lib.xg_qk_norm_rope(p, k, p, p, p, p, 2, H, Hkv, 4, 64, st, st, st, st, r or rotary(), 1e-6, 0, 2, w_dtype, None)
+        return lib.xg_qk_norm_rope(p, k, p, p, p, p, 2, H, Hkv, 4, 64, st, st, st, st, r or rotary(), 1e-6, 2, w_dtype, None)
 
     assert qk(H=0, Hkv=0) == 0 and qk(k=None) == -4 and qk(w_dtype=1) == -1 and qk(H=-1) == -2
 

@@ -165,7 +165,7 @@ _SIGNATURES = {
     "xg_rope_axes": (c_int, [c_void_p] * 2 + [c_int64] * 4 + [ctypes.POINTER(c_int64)] * 2 + [ctypes.POINTER(XgRotary), c_int, c_int, c_void_p]),
     "xg_qk_norm_rope": (
         c_int,
-        [c_void_p] * 6 + [c_int64] * 5 + [ctypes.POINTER(c_int64)] * 4 + [ctypes.POINTER(XgRotary), c_float, c_int, c_int, c_int, c_void_p],
+        [c_void_p] * 6 + [c_int64] * 5 + [ctypes.POINTER(c_int64)] * 4 + [ctypes.POINTER(XgRotary), c_float, c_int, c_int, c_void_p],
     ),
     "xg_qk_norm_rope_bwd_workspace_floats": (c_int64, [c_int64] * 5),
     "xg_qk_norm_rope_bwd": (

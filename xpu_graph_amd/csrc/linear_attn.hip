@@ -900,7 +900,7 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
     gs.S = (int)S;
     gs.D = (int)D;
     gs.group = group;
-    if ((gs.n + 255) / 256 > 0x7fffffffLL) return XG_ERR_TOO_LARGE;
+    if (gs.n > 0xffffff00LL) return XG_ERR_TOO_LARGE;  // threads of a launch
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (int rc = launch_any(p, 3, D, dtype, st)) return rc;

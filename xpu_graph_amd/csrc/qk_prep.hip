@@ -15,7 +15,7 @@
 // partners of the upper half (or two neighbouring vectors of the part that is not rotated), so a row of D elements
 // takes D/16 lanes (rounded up to a power of two for the row sums, which stay inside the wavefront), and a thread
 // takes kHeads heads of one token, which share the table row.  Queries and keys go out in one launch.  All sums and
-// the rotation are fp32; one rounding per output (two with `round_norm`, which rounds n as a separate norm op does).
+// the rotation are fp32; one rounding per output.
 #include "xg_common.hpp"
 
 namespace xg {
@@ -55,7 +55,7 @@ struct Prep {
   int64_t ps[3];               // strides of positions: axis, batch, token
   int64_t table_stride, table_rows;
   int half_off;                // columns from a pair's lower to its upper table entry (0: one entry per pair)
-  int table_f32, w_f32, pos_64, axes, transpose, round_norm;
+  int table_f32, w_f32, pos_64, axes, transpose;
   int D, R, tpr_log2;
   uint32_t units, n_chunks;
   FastDiv by_chunks, by_s;
@@ -223,10 +223,6 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
       for (int e = 0; e < 8; ++e) {
         xl[e] = xl[e] * r * wl[e];
         xh[e] = xh[e] * r * wh[e];
-      }
-      if (p.round_norm) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) xl[e] = to_f32(from_f32<T>(xl[e])), xh[e] = to_f32(from_f32<T>(xh[e]));
       }
     }
     if (!live || h0 + i >= sd.H) continue;
@@ -469,8 +465,9 @@ int launch_prep(Prep& p, int64_t tokens, hipStream_t stream) {
   p.n_chunks = (uint32_t)(p.side[0].chunks + p.side[1].chunks);
   p.by_chunks = FastDiv(p.n_chunks);
   p.units = (uint32_t)(tokens * p.n_chunks);
-  const uint32_t per_block = 256u >> p.tpr_log2;
-  hipLaunchKernelGGL((prep_kernel<T, NORM, FULL, kHeads>), dim3((p.units + per_block - 1) / per_block), dim3(256), 0, stream, p);
+  const uint32_t per_block = 256u >> p.tpr_log2, blocks = (p.units + per_block - 1) / per_block;
+  if (blocks > 0xffffff) return XG_ERR_TOO_LARGE;  // 2^32 threads
+  hipLaunchKernelGGL((prep_kernel<T, NORM, FULL, kHeads>), dim3(blocks), dim3(256), 0, stream, p);
   return status_from_hip(hipGetLastError());
 }
 
@@ -531,7 +528,7 @@ extern "C" int xg_rope_axes(const void* x, void* out, int64_t B, int64_t H, int6
 extern "C" int xg_qk_norm_rope(const void* q, const void* k, const void* q_w, const void* k_w, void* q_out, void* k_out, int64_t B,
                                int64_t H, int64_t Hkv, int64_t S, int64_t D, const int64_t q_strides[3], const int64_t k_strides[3],
                                const int64_t qo_strides[3], const int64_t ko_strides[3], const xg_rotary* rotary, float eps,
-                               int round_norm, int dtype, int w_dtype, xg_stream_t stream) {
+                               int dtype, int w_dtype, xg_stream_t stream) {
   using namespace xg;
   if (int st = check_sizes(B, H, Hkv, S, D, dtype)) return st;
   if (w_dtype != dtype && w_dtype != XG_F32) return XG_ERR_BAD_DTYPE;
@@ -542,7 +539,6 @@ extern "C" int xg_qk_norm_rope(const void* q, const void* k, const void* q_w, co
   if (int st = fill_side(p.side[1], k, nullptr, k_out, k_w, Hkv, k_strides, nullptr, ko_strides, dtype, false)) return st;
   if (int st = fill_common(p, B, S, D, eps)) return st;
   p.w_f32 = w_dtype == XG_F32;
-  p.round_norm = round_norm != 0;
   return run_prep<true>(p, B * S, dtype, reinterpret_cast<hipStream_t>(stream));
 }
 

@@ -55,12 +55,12 @@ void same_device(const Tensor& first, std::initializer_list<const OptTensor*> ot
     TORCH_CHECK_VALUE(!has(*t) || (*t)->device() == first.device(), "xpu_ops: tensors on different devices (", first.device(), " and ", (*t)->device(), ")");
 }
 
-// Unit last stride, the others multiples of 16 bytes.
+// Unit last stride, the others multiples of 16 bytes (dimensions of size 1 have none that counts).
 bool readable(const Tensor& t) {
   const int64_t per16 = 16 / t.element_size(), n = t.dim();
   if (t.stride(n - 1) != 1) return false;
   for (int64_t i = 0; i + 1 < n; ++i)
-    if (t.stride(i) % per16) return false;
+    if (t.size(i) != 1 && t.stride(i) % per16) return false;
   return true;
 }
 
@@ -87,14 +87,23 @@ Tensor result_like(const Tensor& t) {
 // The tensor, or a copy that the kernels can read.
 Tensor operand(const Tensor& t) {
   Tensor x = readable(t) ? t : t.contiguous();
-  return misaligned(x) ? x.clone() : x;
+  return misaligned(x) ? x.clone(at::MemoryFormat::Contiguous) : x;
 }
 Tensor token_operand(const Tensor& t) {
   Tensor x = operand(t);
-  return x.stride(2) < kMaxPitch ? x : x.contiguous();
+  return x.size(2) == 1 || x.stride(2) < kMaxPitch ? x : x.contiguous();
 }
 
-const int64_t* strides(const Tensor& t) { return t.strides().data(); }
+// Strides as the entry points take them: 0 where a dimension has one element, whatever the tensor says there.
+struct Strides {
+  std::array<int64_t, 4> s{};
+  operator const int64_t*() const { return s.data(); }
+};
+Strides strides(const Tensor& t) {
+  Strides r;
+  for (int64_t i = 0; i < 4; ++i) r.s[i] = t.size(i) == 1 ? 0 : t.stride(i);
+  return r;
+}
 
 // Runs `launch(stream)` on the tensor's device, whatever the current one is.
 template <typename F>
@@ -228,8 +237,7 @@ struct Weights {
 };
 
 std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, const OptTensor& wq, const OptTensor& wk, const Tensor& cos,
-                                        const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps,
-                                        bool round_norm) {
+                                        const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps) {
   check_qk(q_in, k_in, wq, wk);
   const int dtype = code(q_in.scalar_type());
   const Rotary rot(q_in, cos, sin, positions, sections, interleaved);
@@ -239,7 +247,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q_in, const Tensor& k_in, 
   const Weights w(q, wq, wk);
   launch(q, "xg_qk_norm_rope", [&](void* stream) {
     return xg_qk_norm_rope(ptr(q), ptr(k), ptr(w.q), ptr(w.k), ptr(q_out), ptr(k_out), q.size(0), q.size(1), k.size(1), q.size(2), q.size(3),
-                           strides(q), strides(k), strides(q_out), strides(k_out), &rot.r, (float)eps, round_norm, dtype, w.dtype, stream);
+                           strides(q), strides(k), strides(q_out), strides(k_out), &rot.r, (float)eps, dtype, w.dtype, stream);
   });
   return {q_out, k_out};
 }
@@ -300,7 +308,7 @@ void check_linear(const Tensor& q, const Tensor& k, const Tensor& v, const Tenso
 OptTensor state_operand(const OptTensor& s) {
   if (!has(s)) return std::nullopt;
   Tensor t = s->contiguous();
-  return misaligned(t) ? t.clone() : t;
+  return misaligned(t) ? t.clone(at::MemoryFormat::Contiguous) : t;
 }
 OptTensor contiguous(const OptTensor& t) { return has(t) ? OptTensor(t->contiguous()) : std::nullopt; }
 int wide(const OptTensor& lengths) { return has(lengths) && lengths->scalar_type() == at::kLong; }
@@ -382,6 +390,8 @@ c10::TypedOperatorHandle<F> handle(const char* name) {
 }
 
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), "xpu_ops: no forward-mode gradients");
   if (!at::GradMode::is_enabled()) return false;
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
@@ -420,20 +430,20 @@ Tensor rope_axes_autograd(const Tensor& x, const Tensor& cos, const Tensor& sin,
 }
 
 using QkSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&, const Tensor&, const OptTensor&,
-                                         at::IntArrayRef, bool, double, bool);
+                                         at::IntArrayRef, bool, double);
 using QkBwdSig = std::tuple<Tensor, Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, const Tensor&, const Tensor&,
                                                             const Tensor&, const Tensor&, const OptTensor&, at::IntArrayRef, bool, double, bool);
 
 struct QkNormRope : torch::autograd::Function<QkNormRope> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const Tensor& cos,
-                               const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps, bool round_norm) {
+                               const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps) {
     static const auto op = handle<QkSig>("xpu_ops::qk_norm_rope");
     ctx->save_for_backward({q, k, or_undefined(wq), or_undefined(wk), cos, sin, or_undefined(positions)});
     ctx->saved_data["sections"] = sections.vec();
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["eps"] = eps;
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [oq, ok] = op.call(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm);
+    auto [oq, ok] = op.call(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps);
     return {oq, ok};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
@@ -444,22 +454,21 @@ struct QkNormRope : torch::autograd::Function<QkNormRope> {
     const bool need_wq = s[2].defined() && ctx->needs_input_grad(2), need_wk = s[3].defined() && ctx->needs_input_grad(s[2].defined() ? 3 : 2);
     auto [dq, dk, gwq, gwk] = op.call(s[0], s[1], or_none(s[2]), or_none(s[3]), g[0], g[1], s[4], s[5], or_none(s[6]), sections,
                                       ctx->saved_data["interleaved"].toBool(), ctx->saved_data["eps"].toDouble(), need_wq || need_wk);
-    return {dq, dk, need_wq ? gwq : Tensor(), need_wk ? gwk : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    return {dq, dk, need_wq ? gwq : Tensor(), need_wk ? gwk : Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
   }
 };
 
 std::tuple<Tensor, Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTensor& wk, const Tensor& cos,
-                                                 const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps,
-                                                 bool round_norm) {
+                                                 const Tensor& sin, const OptTensor& positions, at::IntArrayRef sections, bool interleaved, double eps) {
   TORCH_CHECK_NOT_IMPLEMENTED(!wants_grad({&cos, &sin}), "xpu_ops::qk_norm_rope: no gradient for the cos / sin tables");
   const Tensor uq = or_undefined(wq), uk = or_undefined(wk);
   if (wants_grad({&q, &k, &uq, &uk})) {
-    auto out = QkNormRope::apply(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm);
+    auto out = QkNormRope::apply(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps);
     return {out[0], out[1]};
   }
   static const auto op = handle<QkSig>("xpu_ops::qk_norm_rope");
   at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps, round_norm);
+  return op.call(q, k, wq, wk, cos, sin, positions, sections, interleaved, eps);
 }
 
 using LinSig = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, double);

@@ -1233,14 +1233,14 @@ _library.impl("rope", _rope_meta, "Meta")
 #   axis 0's and so on; interleaved: pair i belongs to axis i % n while i < n * sections[i % n], and to axis 0 from there on.
 #   Without sections: one axis, R = D.  cos / sin: [P, R/2] (a column per pair) or [P, R] (one per element).  positions:
 #   [axes, B, S] (one axis: also [B, S], [S]; None: row s, or the only row).  A position outside the tables gives NaN.
-# qk_norm_rope: RMS norm over each head of q and of k, then that rotation, in one launch for both.  round_norm rounds the
-#   normalised rows to the tensors' dtype before they turn, as rms_norm followed by rope does.
+# qk_norm_rope: RMS norm over each head of q and of k, then that rotation, in one launch for both.  The normalised rows stay
+#   fp32 up to the rotation: one rounding per output, where rms_norm followed by rope rounds twice.
 # rope_axes_bwd, qk_norm_rope_bwd: their gradients (of x; of q, k and the weights, empty where not wanted).
 _library.define("rope_axes(Tensor x, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
 _library.define("rope_axes_bwd(Tensor gy, Tensor cos, Tensor sin, Tensor? positions, int[] sections, bool interleaved=False) -> Tensor")
 _library.define(
     "qk_norm_rope(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor cos, Tensor sin, Tensor? positions, int[] sections, "
-    "bool interleaved, float eps, bool round_norm=False) -> (Tensor, Tensor)"
+    "bool interleaved, float eps) -> (Tensor, Tensor)"
 )
 _library.define(
     "qk_norm_rope_bwd(Tensor q, Tensor k, Tensor? q_weight, Tensor? k_weight, Tensor gq, Tensor gk, Tensor cos, Tensor sin, Tensor? positions, "
@@ -1255,7 +1255,7 @@ def _result_meta(t):
     """A result in the layout of t where the kernels read that in place and it is dense, else contiguous.  (The real ops copy an
     unaligned tensor in its own layout, so alignment does not change it.)"""
     per16 = 16 // t.element_size()
-    if t.stride(-1) == 1 and all(st % per16 == 0 for st in t.stride()[:-1]):
+    if t.stride(-1) == 1 and all(st % per16 == 0 or n == 1 for st, n in zip(t.stride()[:-1], t.shape)):
         return _empty_like_layout(t)
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
@@ -1308,7 +1308,7 @@ def _qk_check(q, k, q_weight, k_weight):
             raise ValueError("qk_norm_rope: a weight is one row of the head dim")
 
 
-def _qk_norm_rope_meta(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps, round_norm=False):
+def _qk_norm_rope_meta(q, k, q_weight, k_weight, cos, sin, positions, sections, interleaved, eps):
     _qk_check(q, k, q_weight, k_weight)
     _rotary_check(q, cos, sin, positions, sections)
     return _result_meta(q), _result_meta(k)
