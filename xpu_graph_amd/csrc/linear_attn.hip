@@ -204,10 +204,12 @@ struct Mover {
   static constexpr int RB = D * 2;
   const char* next;                            // the lowest address of the next whole chunk
   int64_t row_bytes;                           // signed: a reversed operand walks backwards
+  int64_t step;                                // from chunk to chunk
   uint32_t off[2];                             // this lane's part of a tile, from its lowest address
 
   __device__ __forceinline__ void bind(const Operand& o, int b, int head, int len, int reverse, int t0, int tid) {
     row_bytes = (reverse ? -o.s[2] : o.s[2]) * 2;
+    step = C * row_bytes;
     const int64_t lowest = reverse ? (int64_t)(len - 1 - t0) - (C - 1) : (int64_t)t0;
     next = reinterpret_cast<const char*>(o.p) + (b * o.s[0] + (head / o.group) * o.s[1] + lowest * o.s[2]) * 2;
     const uint32_t pitch = (uint32_t)(o.s[2] * 2);
@@ -227,7 +229,7 @@ struct Mover {
     const void* from = (const void*)(uintptr_t)((uint64_t)hi << 32 | lo);
     load_to_lds16(from, off[0], to);
     load_to_lds16(from, off[1], to + 1024);
-    next += C * row_bytes;
+    next += step;
   }
   // the last n < 32 tokens, zeros behind them
   __device__ __forceinline__ void load_tail(int n, char* tile, int tid) const {
@@ -251,15 +253,15 @@ __device__ __forceinline__ void chunk_barrier() {
 
 // S += sum_j x_j k_j on this wave's 32 columns, x[t][jj] the weighed value of the token in slot jj of k-step t.
 // Three bf16 parts of x where the state is a result (`whole`), two where it only feeds O.
-template <typename T, int D, int AT>
-__device__ __forceinline__ void add_to_state(f32x16 (&S)[D / 32], const ColAddresses<T, D>& at, float (&x)[2][8], bool whole) {
+template <typename T, int D>
+__device__ __forceinline__ void add_to_state(f32x16 (&S)[D / 32], const typename Vec8<T>::type (&kc)[2][D / 32], float (&x)[2][8], bool whole) {
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const Parts<2> xv = split<2>(x[t]);
     Parts<kParts<T>> kf[D / 32];
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt) {
-      kf[dt] = as_parts<T>(Tile<T, D>::col_frag(at.k_lo[dt] + AT + 16 * t * Tile<T, D>::RB, at.k_hi[dt] + AT + 16 * t * Tile<T, D>::RB));
+      kf[dt] = as_parts<T>(kc[t][dt]);
       S[dt] = mma_parts(kf[dt], xv, S[dt]);
     }
     if (whole) {
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   typedef Tile<T, D> TL;
   constexpr int STAGE = 2 * TL::BYTES;
   __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of K, V
-  const Problem& pr = p.pr[blockIdx.y];
+  const Problem& pr = p.pr[2 * blockIdx.y];  // dk's states are dv's transposed
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = blockIdx.x % heads;  // neighbours in a token run side by side
@@ -307,12 +309,13 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const int t_beg = seg * p.seg_chunks * C, t_end = t_beg + p.seg_chunks * C;
   if (t_end >= len) return;  // nothing comes after
   const float g2 = head_log2(p, head);
-  int t0 = t_beg;
+  int t_first = t_beg;
   if (g2 < 0.f) {
     const float live = 150.f / -g2;
-    if (live < (float)(t_end - t_beg)) t0 = max(t_beg, t_end - ((int)live / C + 1) * C);
+    if (live < (float)(t_end - t_beg)) t_first = max(t_beg, t_end - ((int)live / C + 1) * C);
   }
-  t0 = __builtin_amdgcn_readfirstlane(t0);
+  t_first = __builtin_amdgcn_readfirstlane(t_first);
+  int t0 = t_end - C;
   f32x16 S[D / 32];
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt)
@@ -321,6 +324,8 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   Mover<T, D> km, vm;
   km.bind(pr.k, b, head, len, pr.reverse, t0, tid);
   vm.bind(pr.v, b, head, len, pr.reverse, t0, tid);
+  km.step = -km.step;
+  vm.step = -vm.step;
   float f[2][8];
   token_factors(f, g2, C, pr.e, pr.s_state, h);
   const uint32_t lds = lds_address(smem);
@@ -334,7 +339,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   auto step = [&](auto stage) {
     constexpr int AT = decltype(stage)::value * STAGE;
     chunk_barrier<0>();
-    if (t0 + C < t_end) issue(STAGE - AT);
+    if (t0 > t_first) issue(STAGE - AT);
     const float rest = decay(g2, t_end - t0 - C);
     float x[2][8];
 #pragma unroll
@@ -343,12 +348,18 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
       for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[jj] * (f[t][jj] * rest);
     }
-    add_to_state<T, D, AT>(S, at, x, true);
-    t0 += C;
+    typename TL::V8 kc[2][D / 32];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+        kc[t][dt] = TL::col_frag(at.k_lo[dt] + AT + 16 * t * TL::RB, at.k_hi[dt] + AT + 16 * t * TL::RB);
+    add_to_state<T, D>(S, kc, x, true);
+    t0 -= C;
   };
-  while (t0 < t_end) {
+  while (t0 >= t_first) {
     step(std::integral_constant<int, 0>{});
-    if (t0 < t_end) step(std::integral_constant<int, 1>{});
+    if (t0 >= t_first) step(std::integral_constant<int, 1>{});
   }
   float* to = pr.seg_states + ((int64_t)bh * p.n_seg + seg) * (D * D);
 #pragma unroll
@@ -361,7 +372,8 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 // Segment states in order: what segment m added becomes the state before segment m.  One thread per four elements.
 template <int D>
 __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
-  const Problem& pr = p.pr[blockIdx.y];
+  const Problem& pr = p.pr[2 * blockIdx.y];
+  float* transposed = blockIdx.y == 0 && p.pr[1].out ? p.pr[1].seg_states : nullptr;
   constexpr int PER = D * D / 1024;  // blocks per head
   const int bh = blockIdx.x / PER;
   const int at = (blockIdx.x % PER) * 1024 + threadIdx.x * 4;
@@ -384,12 +396,36 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
     f32x4 own = {0.f, 0.f, 0.f, 0.f};
     if (!last) own = *cell;
     *cell = S;
+    if (transposed) {  // element (dv, dk + r) of that problem's state
+      const int slot = ((dk / 32 * (D / 32) + dv / 32) * 4 + 2 * ((dv >> 4) & 1) + ((dv >> 2) & 1)) * 64 + 32 * ((dv >> 3) & 1);
+      float* to = transposed + ((int64_t)bh * p.n_seg + m) * (D * D) + (dv & 3);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) to[(slot + sigma((dk + r) & 31)) * 4] = S[r];
+    }
     S = S * decay(g2, seg_len) + own;
   }
   if (len == 0 && pr.state_out) {  // otherwise the last segment ends with it
     float* so = pr.state_out + (int64_t)bh * (D * D);
 #pragma unroll
     for (int r = 0; r < 4; ++r) so[(dk + r) * D + dv] = S[r];
+  }
+}
+
+// Which problem, and which of its n blocks, block i is.  dv and dk of a head read the same rows of q and do in the same order:
+// they are started together on one XCD (blocks go to the eight of them in turn), whose L2 then serves one of the two.
+__device__ __forceinline__ void block_of(const Params& p, int i, int n, int& problem, int& block) {
+  if (!p.pr[1].out || i >= 2 * n) {
+    problem = i < n ? 0 : 2;
+    block = i < n ? i : i - 2 * n;
+    return;
+  }
+  const int whole = n & ~7, rest = n - whole;
+  if (i < 2 * whole) {
+    problem = (i >> 3) & 1;
+    block = ((i >> 4) << 3) + (i & 7);
+  } else {
+    problem = i - 2 * whole >= rest;
+    block = i - whole - problem * rest;
   }
 }
 
@@ -401,10 +437,13 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   constexpr int OP = kParts<T>;  // parts of S and P as operands of O
   constexpr int STAGE = 3 * TL::BYTES;
   extern __shared__ __attribute__((aligned(1024))) char smem[];  // stages of Q, K, V
-  const Problem& pr = p.pr[blockIdx.y];
+  const int heads = p.B * p.H;
+  int problem, at_block;
+  block_of(p, blockIdx.x, heads * p.n_seg, problem, at_block);
+  const Problem& pr = p.pr[problem];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = blockIdx.x % heads;  // neighbours in a token run side by side
+  const int seg = at_block / heads, bh = at_block % heads;  // neighbours in a token run side by side
   const int b = bh / p.H, head = bh % p.H;
   const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C;
@@ -509,8 +548,10 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     auto step = [&](auto stage, int t0) {
       constexpr int AT = decltype(stage)::value * STAGE;
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      if (STAGES == 2 || t0 + C >= t_end)
+      if ((STAGES == 2 && t0 == t_beg) || (STAGES > 2 && t0 + C >= t_end))
         chunk_barrier<0>();
+      else if (STAGES == 2)  // the stores of the chunk before have been issued since
+        chunk_barrier<2>();
       else if (t0 < t_beg + 2 * C)  // the next chunk's six loads have been issued since
         chunk_barrier<6>();
       else  // and the stores (two or more) of one chunk at least
@@ -518,22 +559,40 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       if (t0 + (STAGES - 1) * C < t_end) issue(t0 + (STAGES - 1) * C, (AT + (STAGES - 1) * STAGE) % (STAGES * STAGE));
 
       // P^T = K Q^T and O^T = S^T Q^T from the same rows of Q; each query of O scaled by its decay
+      constexpr int AHEAD = kParts<T> == 1 ? 4 : 2;
+      V8 qr[AHEAD], kr[AHEAD], vf[2], kc[2][D / 32];
+#pragma unroll
+      for (int t = 0; t < AHEAD; ++t) {
+        qr[t] = TL::row_frag(row_at[t] + AT);
+        kr[t] = TL::row_frag(row_at[t] + AT + TL::BYTES);
+      }
+      __builtin_amdgcn_sched_barrier(0);
       f32x16 P, O;
 #pragma unroll
       for (int i = 0; i < 16; ++i) P[i] = O[i] = 0.f;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        const V8 qf = TL::row_frag(row_at[t] + AT);
-        P = mma(TL::row_frag(row_at[t] + AT + TL::BYTES), qf, P);
+        P = mma(kr[t % AHEAD], qr[t % AHEAD], P);
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = S[t >> 1][8 * (t & 1) + i];
-        O = mma_parts(split<OP>(x), as_parts<T>(qf), O);
+        O = mma_parts(split<OP>(x), as_parts<T>(qr[t % AHEAD]), O);
+        __builtin_amdgcn_sched_barrier(0);
+        if (t + AHEAD < D / 16) {
+          qr[t % AHEAD] = TL::row_frag(row_at[t + AHEAD] + AT);
+          kr[t % AHEAD] = TL::row_frag(row_at[t + AHEAD] + AT + TL::BYTES);
+        } else if (t + AHEAD < D / 16 + 2) {
+          const int i = t + AHEAD - D / 16;
+          vf[i] = TL::col_frag(at.v_lo + AT + 16 * i * TL::RB, at.v_hi + AT + 16 * i * TL::RB);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      O *= row_f;
-      V8 vf[2];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) vf[t] = TL::col_frag(at.v_lo + AT + 16 * t * TL::RB, at.v_hi + AT + 16 * t * TL::RB);
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; ++dt)
+          kc[t][dt] = TL::col_frag(at.k_lo[dt] + AT + 16 * t * TL::RB, at.k_hi[dt] + AT + 16 * t * TL::RB);
+      O *= row_f;
 
       // O^T += V^T P^T
 #pragma unroll
@@ -576,7 +635,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int jj = 0; jj < 8; ++jj) x[t][jj] = (float)vf[t][jj] * f[t][jj];
-        add_to_state<T, D, AT>(S, at, x, keep_state);
+        add_to_state<T, D>(S, kc, x, keep_state);
       }
     };
     for (int t0 = t_beg; t0 < t_end; t0 += STAGES * C) {
@@ -734,10 +793,11 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
   constexpr int STAGE = 3 * Tile<T, D>::BYTES;
-  const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), block(D * 2);
+  const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), all(grid.x * grid.y), block(D * 2);
   if (p.n_seg > 1) {
-    hipLaunchKernelGGL((segment_states_kernel<T, D>), grid, block, 0, st, p);
-    hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), (unsigned)n_problems), dim3(256), 0, st, p);
+    const unsigned sums = n_problems == 1 ? 1 : 2;
+    hipLaunchKernelGGL((segment_states_kernel<T, D>), dim3(grid.x, sums), block, 0, st, p);
+    hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), sums), dim3(256), 0, st, p);
   }
   // A third chunk in flight helps where workgroups of the backward end up alone on their compute unit (D 128 bf16 backward:
   // B8 S2048 H32 366 -> 334 us, B8 S4096 H32 727 -> 663; B4 S2048 H32 161 -> 164) and costs a little elsewhere (forward B1 S32768
@@ -745,9 +805,9 @@ int launch(const Params& p, int n_problems, hipStream_t st) {
   if (n_problems > 1 && p.n_seg == 1) {
     auto kernel = linear_attn_kernel<T, D, 3>;
     if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 3 * STAGE)) return rc;
-    hipLaunchKernelGGL(kernel, grid, block, 3 * STAGE, st, p);
+    hipLaunchKernelGGL(kernel, all, block, 3 * STAGE, st, p);
   } else {
-    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), grid, block, 2 * STAGE, st, p);
+    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), all, block, 2 * STAGE, st, p);
   }
   return status_from_hip(hipGetLastError());
 }
@@ -848,7 +908,7 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   const int64_t seg_floats = state_floats(B * H, 3, S, D);
   float* partial = workspace + 3 * seg_floats;
   // dq = scale F(do, v, k), its state the transpose of the forward's
-  Problem& a = p.pr[0];
+  Problem& a = p.pr[2];
   a.q = og;
   a.k = ov;
   a.v = ok;
@@ -859,7 +919,7 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   a.s_intra = a.s_inter = scale;
   a.s_state = 1.f;
   // dv = F_rev(k, q, do): its state ends as the gradient of the initial state
-  Problem& c = p.pr[1];
+  Problem& c = p.pr[0];
   c.q = ok;
   c.k = oq;
   c.v = og;
@@ -868,7 +928,7 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   c.state0 = d_state_out;
   c.state_out = d_state;
   // dk = F_rev(v, do, q): the transposed state
-  Problem& d = p.pr[2];
+  Problem& d = p.pr[1];
   d.q = ov;
   d.k = og;
   d.v = oq;
@@ -885,7 +945,7 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   GroupSum gs{};
   if (group > 1) {
     for (int i = 0; i < 2; ++i) {
-      Problem& r = p.pr[1 + i];
+      Problem& r = p.pr[i];
       gs.part[i] = partial + i * B * H * S * D;
       gs.out[i] = r.out;
       for (int j = 0; j < 3; ++j) gs.os[i][j] = r.os[j];
