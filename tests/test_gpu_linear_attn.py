@@ -154,7 +154,7 @@ def test_without_states(device, dtype, D, state, d_state):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("B,H,Hkv,S,D", [(1, 6, 2, 70, 64), (2, 8, 1, 333, 128), (1, 12, 4, 129, 128), (3, 2, 1, 1, 64)])
+@pytest.mark.parametrize("B,H,Hkv,S,D", [(1, 6, 2, 70, 64), (2, 8, 1, 333, 128), (1, 12, 4, 129, 128), (3, 2, 1, 1, 64), (4, 4, 2, 333, 64), (2, 16, 4, 70, 128)])
 def test_shared_heads(device, dtype, B, H, Hkv, S, D):
     run_all(device, dtype, B, H, Hkv, S, D)
 

@@ -73,6 +73,7 @@ struct Params {
   int len64;
   int B, H, S;
   int n_seg, seg_chunks;
+  int group;                // query heads of a key head that are eight blocks apart (see head_of)
 };
 
 // Row of an accumulator tile (or lane of an operand) -> row of S, column of V: bits 2 and 3 change places.
@@ -292,6 +293,15 @@ __device__ __forceinline__ void token_factors(float (&f)[2][8], float g2, int n,
 __device__ __forceinline__ int state_row(int dt, int g, int h) { return 32 * dt + 16 * (g >> 1) + 8 * h + 4 * (g & 1); }
 __device__ __forceinline__ int state_col(int w, int lane) { return 32 * w + sigma(lane & 31); }
 
+// The head (b H + h) of a block.  Neighbours in a token run side by side; the query heads of one key head are eight blocks apart,
+// which is one XCD (blocks go to the eight in turn), whose L2 serves their reads of K and V.  (D 128, 8 key heads of 32: forward
+// B8 S4096 225 -> 217 us, B1 S32768 286 -> 280, backward B8 S2048 421 -> 412.)
+__device__ __forceinline__ int head_of(const Params& p, int i) {
+  if (p.group == 1) return i;
+  const int span = 8 * p.group, at = i % span;
+  return i - at + (at & 7) * p.group + (at >> 3);
+}
+
 // Each segment's own state (from zero), in accumulator order; that of the last one is not needed, so segments are whole here.
 // Every token is weighed for the end of the segment at once.  Chunks whose weights are all zero in fp32 (lam^n below 2^-150) add
 // nothing and are not read.
@@ -303,7 +313,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const Problem& pr = p.pr[2 * blockIdx.y];  // dk's states are dv's transposed
   const int tid = threadIdx.x, lane = tid & 63, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = blockIdx.x % heads;  // neighbours in a token run side by side
+  const int heads = p.B * p.H, seg = blockIdx.x / heads, bh = head_of(p, blockIdx.x % heads);
   const int b = bh / p.H, head = bh % p.H;
   const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C, t_end = t_beg + p.seg_chunks * C;
@@ -429,21 +439,20 @@ __device__ __forceinline__ void block_of(const Params& p, int i, int n, int& pro
   }
 }
 
-// STAGES: chunks of tiles in LDS.
-template <typename T, int D, int STAGES>
+template <typename T, int D>
 __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) void linear_attn_kernel(const Params p) {
   typedef typename Vec8<T>::type V8;
   typedef Tile<T, D> TL;
   constexpr int OP = kParts<T>;  // parts of S and P as operands of O
   constexpr int STAGE = 3 * TL::BYTES;
-  extern __shared__ __attribute__((aligned(1024))) char smem[];  // stages of Q, K, V
+  __shared__ __attribute__((aligned(1024))) char smem[2 * STAGE];  // two stages of Q, K, V
   const int heads = p.B * p.H;
   int problem, at_block;
   block_of(p, blockIdx.x, heads * p.n_seg, problem, at_block);
   const Problem& pr = p.pr[problem];
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int seg = at_block / heads, bh = at_block % heads;  // neighbours in a token run side by side
+  const int seg = at_block / heads, bh = head_of(p, at_block % heads);
   const int b = bh / p.H, head = bh % p.H;
   const int len = __builtin_amdgcn_readfirstlane(length_of(p, b));
   const int t_beg = seg * p.seg_chunks * C;
@@ -520,7 +529,6 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       }
     };
     issue(t_beg, 0);
-    if (STAGES > 2 && t_beg + C < t_end) issue(t_beg + C, STAGE);
 
     // what does not change from chunk to chunk: factors, addresses
     float f[2][8];
@@ -548,17 +556,15 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     auto step = [&](auto stage, int t0) {
       constexpr int AT = decltype(stage)::value * STAGE;
       const int n = t_end - t0 < C ? t_end - t0 : C;
-      if ((STAGES == 2 && t0 == t_beg) || (STAGES > 2 && t0 + C >= t_end))
+      if (t0 == t_beg)
         chunk_barrier<0>();
-      else if (STAGES == 2)  // the stores of the chunk before have been issued since
+      else  // two stores or more of the chunk before have been issued since
         chunk_barrier<2>();
-      else if (t0 < t_beg + 2 * C)  // the next chunk's six loads have been issued since
-        chunk_barrier<6>();
-      else  // and the stores (two or more) of one chunk at least
-        chunk_barrier<8>();
-      if (t0 + (STAGES - 1) * C < t_end) issue(t0 + (STAGES - 1) * C, (AT + (STAGES - 1) * STAGE) % (STAGES * STAGE));
+      if (t0 + C < t_end) issue(t0 + C, STAGE - AT);
 
       // P^T = K Q^T and O^T = S^T Q^T from the same rows of Q; each query of O scaled by its decay
+      // (rows are read AHEAD k-steps before they are used, where the compiler would wait for each pair: a chunk of one wave a SIMD
+      // takes 1.38 us instead of 1.5; fp16's parts leave registers for two)
       constexpr int AHEAD = kParts<T> == 1 ? 4 : 2;
       V8 qr[AHEAD], kr[AHEAD], vf[2], kc[2][D / 32];
 #pragma unroll
@@ -638,11 +644,9 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         add_to_state<T, D>(S, kc, x, keep_state);
       }
     };
-    for (int t0 = t_beg; t0 < t_end; t0 += STAGES * C) {
-      sdpa::static_for<STAGES>([&](auto stage) {
-        constexpr int i = decltype(stage)::value;
-        if (i == 0 || t0 + i * C < t_end) step(stage, t0 + i * C);
-      });
+    for (int t0 = t_beg; t0 < t_end; t0 += 2 * C) {
+      step(std::integral_constant<int, 0>{}, t0);
+      if (t0 + C < t_end) step(std::integral_constant<int, 1>{}, t0 + C);
     }
   }
 
@@ -746,10 +750,15 @@ constexpr int64_t kMaxPitch = 1 << 26;  // elements between tokens: 32 rows stay
 
 int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
 
-// How many segments the tokens of a head are cut into: enough workgroups to fill the chip twice over, at least four chunks each.
-void segments(int64_t heads, int64_t n_problems, int64_t S, int& n_seg, int& seg_chunks) {
-  const int64_t chunks = chunks_of(S), groups = heads * n_problems;
-  int64_t n = groups >= 256 ? 1 : (512 + groups - 1) / groups;
+// How many segments the tokens of a head are cut into, four chunks at least each.  Cutting reads K and V twice; not cutting leaves
+// the chip idle where there are few heads, each of which takes 1.4 us a chunk.  Up to half the heads that fill it with one wave a
+// SIMD they are cut to fill it once, or twice where that would be less than four segments.  Measured (bf16 D 128, us, uncut /
+// segments: once, twice the chip): forward 32 heads S 32768 1362 / 8: 336, 16: 356; 64 heads S 8192 339 / 4: 179, 8: 182; 96 heads
+// S 4096 174 / 2: 147, 5: 129; 128 heads S 2048 99 / 2: 96, 4: 92; 192 heads S 2048 109 / 2: 132, 3: 145; backward (three times the
+// heads) 32 heads S 32768 1242 / 2: 1007, 5: 790, 64 heads S 8192 348 / 2: 398.
+void segments(int64_t heads, int64_t n_problems, int64_t S, int64_t D, int& n_seg, int& seg_chunks) {
+  const int64_t chunks = chunks_of(S), groups = heads * n_problems, full = 256 * (128 / D);
+  int64_t n = groups > full / 2 ? 1 : (full / groups >= 4 ? full : 2 * full) / groups;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   seg_chunks = (int)((chunks + n - 1) / n);
@@ -759,7 +768,7 @@ void segments(int64_t heads, int64_t n_problems, int64_t S, int& n_seg, int& seg
 // Floats of the segment states of one problem.
 int64_t state_floats(int64_t heads, int64_t n_problems, int64_t S, int64_t D) {
   int n_seg, seg_chunks;
-  segments(heads, n_problems, S, n_seg, seg_chunks);
+  segments(heads, n_problems, S, D, n_seg, seg_chunks);
   return n_seg > 1 ? heads * n_seg * D * D : 0;
 }
 
@@ -792,23 +801,13 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
 
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
-  constexpr int STAGE = 3 * Tile<T, D>::BYTES;
   const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), all(grid.x * grid.y), block(D * 2);
   if (p.n_seg > 1) {
     const unsigned sums = n_problems == 1 ? 1 : 2;
     hipLaunchKernelGGL((segment_states_kernel<T, D>), dim3(grid.x, sums), block, 0, st, p);
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), sums), dim3(256), 0, st, p);
   }
-  // A third chunk in flight helps where workgroups of the backward end up alone on their compute unit (D 128 bf16 backward:
-  // B8 S2048 H32 366 -> 334 us, B8 S4096 H32 727 -> 663; B4 S2048 H32 161 -> 164) and costs a little elsewhere (forward B1 S32768
-  // H32 359 -> 364, B8 S4096 H32 249 -> 252).
-  if (n_problems > 1 && p.n_seg == 1) {
-    auto kernel = linear_attn_kernel<T, D, 3>;
-    if (int rc = allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 3 * STAGE)) return rc;
-    hipLaunchKernelGGL(kernel, all, block, 3 * STAGE, st, p);
-  } else {
-    hipLaunchKernelGGL((linear_attn_kernel<T, D, 2>), all, block, 2 * STAGE, st, p);
-  }
+  hipLaunchKernelGGL((linear_attn_kernel<T, D>), all, block, 0, st, p);
   return status_from_hip(hipGetLastError());
 }
 
@@ -850,7 +849,8 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
   p.B = (int)B;
   p.H = (int)H;
   p.S = (int)S;
-  segments(B * H, 1, S, p.n_seg, p.seg_chunks);
+  p.group = B * H % (8 * group) == 0 ? group : 1;
+  segments(B * H, 1, S, D, p.n_seg, p.seg_chunks);
   if (p.n_seg > 1) {
     if (!workspace) return XG_ERR_NULL_PTR;
     if (workspace_floats < B * H * p.n_seg * D * D) return XG_ERR_BAD_ARG;
@@ -899,7 +899,8 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   p.B = (int)B;
   p.H = (int)H;
   p.S = (int)S;
-  segments(B * H, 3, S, p.n_seg, p.seg_chunks);
+  p.group = B * H % (8 * group) == 0 ? group : 1;
+  segments(B * H, 3, S, D, p.n_seg, p.seg_chunks);
   const int64_t need = xg_linear_attn_bwd_workspace_floats(B, H, Hkv, S, D);
   if (need) {
     if (!workspace) return XG_ERR_NULL_PTR;
