@@ -30,6 +30,12 @@
 //
 // A few heads do not fill the chip.  The tokens are then cut into segments: one launch sums up each segment's own state, one
 // turns them into the states before each segment (elementwise, in order), and the kernel above runs all segments at once.
+//
+// What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 270 others a chunk), of
+// which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 238 us (1.07 GB, 4.5 TB/s), B8 S2048
+// 122 us, B4 S2048 92 us (four segments: K and V twice, 0.40 GB), B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
+// 580 us, B4 S2048 160 us (0.73 GB by the counters, 4.6 TB/s: seven tensors in where dv and dk share, nearly eight as it runs,
+// three out), B1 S32768 788 us.
 #include "sdpa_common.hpp"
 
 namespace xg {
@@ -400,19 +406,26 @@ __global__ __launch_bounds__(256) void scan_states_kernel(const Params p) {
   }
   float* ws = pr.seg_states + (int64_t)bh * p.n_seg * (D * D) + at;
   const int seg_len = p.seg_chunks * C;
-  for (int m = 0; m * seg_len < len; ++m) {
-    f32x4* cell = reinterpret_cast<f32x4*>(ws + (int64_t)m * (D * D));
-    const bool last = (m + 1) * seg_len >= len;
-    f32x4 own = {0.f, 0.f, 0.f, 0.f};
-    if (!last) own = *cell;
-    *cell = S;
-    if (transposed) {  // element (dv, dk + r) of that problem's state
-      const int slot = ((dk / 32 * (D / 32) + dv / 32) * 4 + 2 * ((dv >> 4) & 1) + ((dv >> 2) & 1)) * 64 + 32 * ((dv >> 3) & 1);
-      float* to = transposed + ((int64_t)bh * p.n_seg + m) * (D * D) + (dv & 3);
+  const float lam = decay(g2, seg_len);
+  constexpr int BATCH = 8;  // loads in flight (32 segments, B1 S8192 H8 D128: forward 48 -> 42 us; four segments: no change)
+  for (int m0 = 0; m0 * seg_len < len; m0 += BATCH) {
+    f32x4 own[BATCH];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) to[(slot + sigma((dk + r) & 31)) * 4] = S[r];
+    for (int i = 0; i < BATCH; ++i)
+      if ((m0 + i + 1) * seg_len < len) own[i] = *reinterpret_cast<const f32x4*>(ws + (int64_t)(m0 + i) * (D * D));
+#pragma unroll
+    for (int i = 0; i < BATCH; ++i) {
+      const int m = m0 + i;
+      if (m * seg_len >= len) break;
+      *reinterpret_cast<f32x4*>(ws + (int64_t)m * (D * D)) = S;
+      if (transposed) {  // element (dv, dk + r) of that problem's state
+        const int slot = ((dk / 32 * (D / 32) + dv / 32) * 4 + 2 * ((dv >> 4) & 1) + ((dv >> 2) & 1)) * 64 + 32 * ((dv >> 3) & 1);
+        float* to = transposed + ((int64_t)bh * p.n_seg + m) * (D * D) + (dv & 3);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) to[(slot + sigma((dk + r) & 31)) * 4] = S[r];
+      }
+      if ((m + 1) * seg_len < len) S = S * lam + own[i];
     }
-    S = S * decay(g2, seg_len) + own;
   }
   if (len == 0 && pr.state_out) {  // otherwise the last segment ends with it
     float* so = pr.state_out + (int64_t)bh * (D * D);
@@ -690,7 +703,7 @@ __global__ __launch_bounds__(256) void group_sum_kernel(const GroupSum p) {
 }
 
 // One token: the state of a head is read, updated and written in place, and the row q S comes out of the same pass.
-// Bound by the state's bytes (two ways).  A workgroup takes 32 columns of one head's state: eight lanes per row (16 bytes each,
+// Bound by the state's bytes (two ways): B64 H32 D128 54 us, 268 MB, 5.0 TB/s; one sequence 3.5 us.  A workgroup takes 32 columns of one head's state: eight lanes per row (16 bytes each,
 // 128-byte lines), 32 rows at a time.
 struct StepParams {
   const void* q;

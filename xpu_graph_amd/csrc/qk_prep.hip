@@ -16,6 +16,9 @@
 // takes D/16 lanes (rounded up to a power of two for the row sums, which stay inside the wavefront), and a thread
 // takes kHeads heads of one token, which share the table row.  Queries and keys go out in one launch.  All sums and
 // the rotation are fp32; one rounding per output.
+// Measured (bf16, D 128): rope_axes B2 S6144 H32, three axes 36 us, 201 MB, 5.6 TB/s; qk_norm_rope B4 S2048 H32/8 34 us, 168 MB,
+// 4.9 TB/s, H32/32 51 us, 268 MB, 5.3 TB/s, its backward 78 + 4 us, 403 MB, 5.0 TB/s.  D 96 leaves two of a row's eight lanes
+// idle: fp16 B3 S1371 H10/5 13 us forward, 18 + 4 us backward.
 #include "xg_common.hpp"
 
 namespace xg {
@@ -88,8 +91,7 @@ __device__ __forceinline__ void load8_as(const void* base, int64_t at, int f32, 
   }
 }
 
-// Sum over the 2^log2 lanes of a row; the same tree whatever the width, so that the lanes of a narrower row add up as
-// the first lanes of a wider one do.
+// Sum over the 2^log2 lanes of a row.
 __device__ __forceinline__ float row_sum(float v, int log2) {
   auto dpp = [](float x, auto CTRL) {
     constexpr int ctrl = decltype(CTRL)::value;
@@ -212,13 +214,10 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) xl[e] = to_f32(lo[i][e]), xh[e] = to_f32(hi[i][e]);
     if constexpr (NORM) {
-      float a = 0.f, c = 0.f;
+      float a = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) a += xl[e] * xl[e];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) c += xh[e] * xh[e];
-      // the two halves add up on their own, as the sixteen lanes of a row do in the norm kernel
-      const float r = rsqrtf((row_sum(a, p.tpr_log2) + row_sum(c, p.tpr_log2)) * p.inv_d + p.eps);
+      for (int e = 0; e < 8; ++e) a += xl[e] * xl[e] + xh[e] * xh[e];
+      const float r = rsqrtf(row_sum(a, p.tpr_log2) * p.inv_d + p.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         xl[e] = xl[e] * r * wl[e];
