@@ -474,8 +474,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   const float g2 = head_log2(p, head);
   const int64_t out0 = b * pr.os[0] + head * pr.os[1];
 
-  // rows behind the sequence: zeros
-  {
+  auto clear_rows_behind = [&] {  // zeros
     const int from = t_beg > len ? t_beg : len;
     for (int idx = tid; idx < (s_end - from) * (D / 8); idx += D * 2) {
       const int64_t at = out0 + (int64_t)(from + idx / (D / 8)) * pr.os[2] + (idx % (D / 8)) * 8;
@@ -488,7 +487,26 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
         *reinterpret_cast<u32x4*>(reinterpret_cast<T*>(pr.out) + at) = zero;
       }
     }
-  }
+  };
+  if (p.n_seg > 1 && t_beg >= t_end) return clear_rows_behind();
+
+  Mover<T, D> qm, km, vm;
+  qm.bind(pr.q, b, head, len, pr.reverse, t_beg, tid);
+  km.bind(pr.k, b, head, len, pr.reverse, t_beg, tid);
+  vm.bind(pr.v, b, head, len, pr.reverse, t_beg, tid);
+  const uint32_t lds = lds_address(smem);
+  auto issue = [&](int t0, int stage_at) {
+    if (t_end - t0 >= C) {
+      const uint32_t to = __builtin_amdgcn_readfirstlane(lds + stage_at + 2048 * w);
+      qm.load(to);
+      km.load(to + TL::BYTES);
+      vm.load(to + 2 * TL::BYTES);
+    } else {
+      qm.load_tail(t_end - t0, smem + stage_at, tid);
+      km.load_tail(t_end - t0, smem + stage_at + TL::BYTES, tid);
+      vm.load_tail(t_end - t0, smem + stage_at + 2 * TL::BYTES, tid);
+    }
+  };
 
   // the state before the segment
   f32x16 S[D / 32];
@@ -497,7 +515,6 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
 #pragma unroll
     for (int i = 0; i < 16; ++i) S[dt][i] = 0.f;
   if (p.n_seg > 1) {
-    if (t_beg >= t_end) return;
     const float* from = pr.seg_states + ((int64_t)bh * p.n_seg + seg) * (D * D);
 #pragma unroll
     for (int dt = 0; dt < D / 32; ++dt)
@@ -510,39 +527,29 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
   } else if (pr.state0) {
     const float* s0 = pr.state0 + (int64_t)bh * (D * D);
     const int dv = state_col(w, lane);
+    if (pr.state0_t) {
 #pragma unroll
-    for (int dt = 0; dt < D / 32; ++dt)
+      for (int dt = 0; dt < D / 32; ++dt)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int dk = state_row(dt, i >> 2, h) + (i & 3);
-        S[dt][i] = pr.state0_t ? s0[dv * D + dk] : s0[dk * D + dv];
-      }
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(s0 + dv * D + state_row(dt, g, h));
+#pragma unroll
+          for (int r = 0; r < 4; ++r) S[dt][4 * g + r] = x[r];
+        }
+    } else {
+#pragma unroll
+      for (int dt = 0; dt < D / 32; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) S[dt][i] = s0[(state_row(dt, i >> 2, h) + (i & 3)) * D + dv];
+    }
   }
-  // the loads above end here: left to the first use, the wait for them would stand inside the loop and hold up its prefetch
+  if (t_beg < t_end) issue(t_beg, 0);
+  // the loads of the state end here: left to the first use, the wait for them would stand inside the loop and hold up its prefetch
 #pragma unroll
   for (int dt = 0; dt < D / 32; ++dt) asm volatile("" : "+v"(S[dt]));
   const bool keep_state = pr.state_out && (p.n_seg == 1 || (t_beg < t_end && t_end == len));  // this segment ends with the last token
 
   if (t_beg < t_end) {
-    Mover<T, D> qm, km, vm;
-    qm.bind(pr.q, b, head, len, pr.reverse, t_beg, tid);
-    km.bind(pr.k, b, head, len, pr.reverse, t_beg, tid);
-    vm.bind(pr.v, b, head, len, pr.reverse, t_beg, tid);
-    const uint32_t lds = lds_address(smem);
-    auto issue = [&](int t0, int stage_at) {
-      if (t_end - t0 >= C) {
-        const uint32_t to = __builtin_amdgcn_readfirstlane(lds + stage_at + 2048 * w);
-        qm.load(to);
-        km.load(to + TL::BYTES);
-        vm.load(to + 2 * TL::BYTES);
-      } else {
-        qm.load_tail(t_end - t0, smem + stage_at, tid);
-        km.load_tail(t_end - t0, smem + stage_at + TL::BYTES, tid);
-        vm.load_tail(t_end - t0, smem + stage_at + 2 * TL::BYTES, tid);
-      }
-    };
-    issue(t_beg, 0);
-
     // what does not change from chunk to chunk: factors, addresses
     float f[2][8];
     token_factors(f, g2, C, pr.e, pr.s_state, h);
@@ -663,6 +670,7 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
     }
   }
 
+  clear_rows_behind();
   if (keep_state) {
     float* so = pr.state_out + (int64_t)bh * (D * D);
     const int dv = state_col(w, lane);
