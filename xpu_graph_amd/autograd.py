@@ -30,7 +30,7 @@ recomputed with one more dense call.  The gated layer saves only its inputs: bot
 dense kernel, the two input-gradient products run as one chain (the second takes the first as its residual).
 
 rope_axes, qk_norm_rope and linear_attn have their formulas beside their implementations in csrc/torch_ops.cpp, always
-registered: in C++ they cost an inference call nothing that could be measured.
+registered: an inference call passes through one C++ function more.
 """
 import torch
 
