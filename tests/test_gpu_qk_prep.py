@@ -416,3 +416,28 @@ def test_gradients_that_do_not_exist_are_refused(device):
     with torch.autograd.forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         z = x.detach()
         _ops().rope_axes(torch.autograd.forward_ad.make_dual(z, z), cos, sin, None, [])
+
+
+@pytest.mark.parametrize("layout", ["heads", "tokens", "packed", "batch inside", "shared", "one head", "odd"])
+def test_results_lie_as_the_shape_functions_say(device, layout):
+    B, H, S, D = 2, 3, 5, 64
+    x = {
+        "heads": lambda: torch.randn(B, H, S, D),
+        "tokens": lambda: torch.randn(B, S, H, D).transpose(1, 2),
+        "packed": lambda: torch.randn(B, S, 3 * H * D).view(B, S, 3 * H, D).transpose(1, 2)[:, H : 2 * H],
+        "batch inside": lambda: torch.randn(S, B, 2 * H, D).permute(1, 2, 0, 3)[:, :H],
+        "shared": lambda: torch.randn(B, 1, S, D).expand(B, H, S, D),
+        "one head": lambda: torch.randn(B, S, 1, D).transpose(1, 2),
+        "odd": lambda: torch.randn(B, S, H, D + 3).transpose(1, 2)[..., 1 : D + 1],
+    }[layout]().bfloat16().to(device)
+    cos, sin = tables(S, D // 2, device, torch.float32, 1, False)
+    args = lambda x, c, s: (x, x, None, None, c, s, None, [], False, 1e-6)  # noqa: E731
+    got = _ops().qk_norm_rope(*args(x, cos, sin))
+    as_meta = lambda t: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device="meta")  # noqa: E731
+    told = _ops().qk_norm_rope(*args(as_meta(x), as_meta(cos), as_meta(sin)))
+    assert [t.stride() for t in got] == [t.stride() for t in told]
+    want = _ops().qk_norm_rope(*args(x.contiguous(), cos, sin))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    lin = lambda x, g: _ops().linear_attn(x, x, x, g, None, None, 1.0)  # noqa: E731
+    g = torch.zeros(x.shape[1], device=device)
+    assert [t.stride() for t in lin(x, g)] == [t.stride() for t in lin(as_meta(x), as_meta(g))]

@@ -73,6 +73,14 @@ def test_layouts_survive():
     assert OPS.rope_axes(x, t, t, None, []).stride() == x.stride()
 
 
+def test_a_part_of_a_projection_gives_results_in_its_order():
+    heads = meta(2, 3, 12 * 64).view(2, 3, 12, 64).transpose(1, 2)
+    t = meta(3, 32, dtype=torch.float32)
+    q, k = OPS.qk_norm_rope(heads[:, :8], heads[:, 8:10], None, None, t, t, None, [], False, 1e-6)
+    assert q.stride() == (3 * 8 * 64, 64, 8 * 64, 1) and k.stride() == (3 * 2 * 64, 64, 2 * 64, 1)
+    assert OPS.rope_axes(heads[:, :1].expand(2, 4, 3, 64), t, t, None, []).is_contiguous()  # shared heads: no order of their own
+
+
 def test_layouts_of_dimensions_of_one_element():
     """What torch keeps as the stride of a dimension of size 1 does not decide about the layout."""
     x = torch.empty(1, 3, 8, 64, device="meta", dtype=torch.bfloat16).as_strided((1, 3, 8, 64), (1 << 40, 64, 192, 1))

@@ -115,22 +115,42 @@ struct Turn {
 
 // The table entries of this thread's eight pairs of token (b, s): one row when they share an axis, else the rows of
 // every axis that occurs, picked per pair.
+__device__ __forceinline__ int64_t table_row(const Prep& p, int a, int b, int s) {
+  if (!p.pos) return s;
+  const int64_t at = a * p.ps[0] + b * p.ps[1] + s * p.ps[2];
+  return p.pos_64 ? reinterpret_cast<const int64_t*>(p.pos)[at] : (int64_t) reinterpret_cast<const int32_t*>(p.pos)[at];
+}
 template <typename T, bool FULL>
 __device__ __forceinline__ void load_turn(const Prep& p, int j, int b, int s, Turn<FULL>& t) {
-  const uint32_t bits = p.axis_bits[j];
-  const int64_t col = 8 * j;
   const float nan = __builtin_nanf("");
+  const int64_t col = 8 * j;
+  if (p.axes == 1) {
+    const int64_t row = table_row(p, 0, b, s);
+    const bool bad = p.pos && (row < 0 || row >= p.table_rows);
+    const int64_t at = (bad ? 0 : row) * p.table_stride + col;
+    load8_as<T>(p.cos, at, p.table_f32, t.cl);
+    load8_as<T>(p.sin, at, p.table_f32, t.sl);
+    if constexpr (FULL) {
+      load8_as<T>(p.cos, at + p.half_off, p.table_f32, t.ch);
+      load8_as<T>(p.sin, at + p.half_off, p.table_f32, t.sh);
+    }
+    if (bad) {  // cos alone makes every element it turns NaN
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        t.cl[e] = nan;
+        if constexpr (FULL) t.ch[e] = nan;
+      }
+    }
+    return;
+  }
+  const uint32_t bits = p.axis_bits[j];
   for (int a = 0; a < p.axes; ++a) {
     uint32_t hit = 0;  // pairs of this axis
 #pragma unroll
     for (int e = 0; e < 8; ++e) hit |= (uint32_t)(((bits >> (2 * e)) & 3u) == (uint32_t)a) << e;
     if (hit == 0) continue;
-    int64_t row = s;
-    if (p.pos) {
-      const int64_t at = a * p.ps[0] + b * p.ps[1] + s * p.ps[2];
-      row = p.pos_64 ? reinterpret_cast<const int64_t*>(p.pos)[at] : (int64_t) reinterpret_cast<const int32_t*>(p.pos)[at];
-    }
-    const bool bad = p.pos && (row < 0 || row >= p.table_rows);
+    const int64_t row = table_row(p, a, b, s);
+    const bool bad = row < 0 || row >= p.table_rows;
     const int64_t at = (bad ? 0 : row) * p.table_stride + col;
     auto pick = [&](const void* table, int64_t from, float (&to)[8]) {
       float x[8];
@@ -174,17 +194,13 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
   columns(p, live ? j : 0, lo_c, hi_c, rotated);
 
   const T* x = reinterpret_cast<const T*>(sd.x) + b * sd.xs[0] + s * sd.xs[2];
+  // loads without a condition, so that all of them are on their way together: a lane or a head too many reads another one's
   V8 lo[kHeads], hi[kHeads];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    if (live && h0 + i < sd.H) {
-      const T* row = x + (int64_t)(h0 + i) * sd.xs[1];
-      lo[i] = *reinterpret_cast<const V8*>(row + lo_c);
-      hi[i] = *reinterpret_cast<const V8*>(row + hi_c);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) lo[i][e] = hi[i][e] = (T)0.f;
-    }
+    const T* row = x + (int64_t)min(h0 + i, sd.H - 1) * sd.xs[1];
+    lo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(row + lo_c));
+    hi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(row + hi_c));
   }
   Turn<FULL> t{};
   if (live && rotated) {
@@ -217,6 +233,7 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
       float a = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) a += xl[e] * xl[e] + xh[e] * xh[e];
+      if (!live) a = 0.f;
       const float r = rsqrtf(row_sum(a, p.tpr_log2) * p.inv_d + p.eps);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -224,21 +241,17 @@ __global__ __launch_bounds__(256) void prep_kernel(const Prep p) {
         xh[e] = xh[e] * r * wh[e];
       }
     }
-    if (!live || h0 + i >= sd.H) continue;
     V8 ol, oh;
-    if (rotated) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ol[e] = from_f32<T>(xl[e] * t.cl[e] - xh[e] * t.sl[e]);
-        oh[e] = from_f32<T>(xh[e] * t.c_hi(e) + xl[e] * t.s_hi(e));
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ol[e] = from_f32<T>(xl[e]), oh[e] = from_f32<T>(xh[e]);
+    for (int e = 0; e < 8; ++e) {
+      ol[e] = from_f32<T>(rotated ? xl[e] * t.cl[e] - xh[e] * t.sl[e] : xl[e]);
+      oh[e] = from_f32<T>(rotated ? xh[e] * t.c_hi(e) + xl[e] * t.s_hi(e) : xh[e]);
     }
-    T* row = out + (int64_t)(h0 + i) * sd.os[1];
-    __builtin_nontemporal_store(ol, reinterpret_cast<V8*>(row + lo_c));
-    __builtin_nontemporal_store(oh, reinterpret_cast<V8*>(row + hi_c));
+    if (live && h0 + i < sd.H) {
+      T* row = out + (int64_t)(h0 + i) * sd.os[1];
+      __builtin_nontemporal_store(ol, reinterpret_cast<V8*>(row + lo_c));
+      __builtin_nontemporal_store(oh, reinterpret_cast<V8*>(row + hi_c));
+    }
   }
 }
 
@@ -278,18 +291,14 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
     T* out = reinterpret_cast<T*>(sd.out) + b * sd.os[0] + s * sd.os[2];
     V8 xlo[kHeads], xhi[kHeads], glo[kHeads], ghi[kHeads];
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-      if (live && h0 + i < sd.H) {
-        const T* xr = x + (int64_t)(h0 + i) * sd.xs[1];
-        const T* gr = g + (int64_t)(h0 + i) * sd.gs[1];
-        xlo[i] = *reinterpret_cast<const V8*>(xr + lo_c);
-        xhi[i] = *reinterpret_cast<const V8*>(xr + hi_c);
-        glo[i] = *reinterpret_cast<const V8*>(gr + lo_c);
-        ghi[i] = *reinterpret_cast<const V8*>(gr + hi_c);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) xlo[i][e] = xhi[i][e] = glo[i][e] = ghi[i][e] = (T)0.f;
-      }
+    for (int i = 0; i < kHeads; ++i) {  // (without a condition, as in the forward)
+      const int head = min(h0 + i, sd.H - 1);
+      const T* xr = x + (int64_t)head * sd.xs[1];
+      const T* gr = g + (int64_t)head * sd.gs[1];
+      xlo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(xr + lo_c));
+      xhi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(xr + hi_c));
+      glo[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(gr + lo_c));
+      ghi[i] = __builtin_nontemporal_load(reinterpret_cast<const V8*>(gr + hi_c));
     }
     Turn<FULL> t{};
     if (live && rotated) load_turn<T, FULL>(p, j, b, s, t);
@@ -303,30 +312,29 @@ __global__ __launch_bounds__(256) void prep_bwd_kernel(const Prep p) {
         gl[e] = rotated ? a * t.cl[e] + c * t.s_hi(e) : a;
         gh[e] = rotated ? c * t.c_hi(e) - a * t.sl[e] : c;
       }
-      if (!live) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) gl[e] = gh[e] = 0.f;
-      }
       float ss = 0.f, sg = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         ss += xl[e] * xl[e] + xh[e] * xh[e];
         sg += gl[e] * wl[e] * xl[e] + gh[e] * wh[e] * xh[e];
       }
+      if (!live) ss = sg = 0.f;
       const float r = rsqrtf(row_sum(ss, p.tpr_log2) * p.inv_d + p.eps);
       const float m = row_sum(sg, p.tpr_log2) * p.inv_d * r * r;  // mean(gn w xhat) r
-      if (!live || h0 + i >= sd.H) continue;
       V8 ol, oh;
+      const bool own = live && h0 + i < sd.H;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         ol[e] = from_f32<T>(r * (gl[e] * wl[e] - xl[e] * m));
         oh[e] = from_f32<T>(r * (gh[e] * wh[e] - xh[e] * m));
-        gwl[e] += gl[e] * xl[e] * r;
-        gwh[e] += gh[e] * xh[e] * r;
+        gwl[e] += own ? gl[e] * xl[e] * r : 0.f;
+        gwh[e] += own ? gh[e] * xh[e] * r : 0.f;
       }
-      T* row = out + (int64_t)(h0 + i) * sd.os[1];
-      __builtin_nontemporal_store(ol, reinterpret_cast<V8*>(row + lo_c));
-      __builtin_nontemporal_store(oh, reinterpret_cast<V8*>(row + hi_c));
+      if (own) {
+        T* row = out + (int64_t)(h0 + i) * sd.os[1];
+        __builtin_nontemporal_store(ol, reinterpret_cast<V8*>(row + lo_c));
+        __builtin_nontemporal_store(oh, reinterpret_cast<V8*>(row + hi_c));
+      }
     }
   }
   if (p.gw_part == nullptr) return;

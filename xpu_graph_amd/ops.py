@@ -1251,12 +1251,24 @@ ROPE_MAX_AXES = 4
 ROPE_MAX_HEAD_DIM = 512
 
 
-def _result_meta(t):
-    """A result in the layout of t where the kernels read that in place and it is dense, else contiguous.  (The real ops copy an
-    unaligned tensor in its own layout, so alignment does not change it.)"""
-    per16 = 16 // t.element_size()
-    if t.stride(-1) == 1 and all(st % per16 == 0 or n == 1 for st, n in zip(t.stride()[:-1], t.shape)):
-        return _empty_like_layout(t)
+_MAX_PITCH = 1 << 26  # elements between tokens that the chunked linear attention kernels address
+
+
+def _result_meta(t, max_pitch=None):
+    """A result in the layout of t where the kernels read that in place and it is dense; dense with the dimensions in the order of
+    t's strides where it is a part of something else; else contiguous.  (As in csrc/torch_ops.cpp; alignment does not change it.)"""
+    if t.stride(-1) == 1 and all(n != 0 for n in t.shape):
+        per16 = 16 // t.element_size()
+        to = list(t.stride())
+        if not (all(st % per16 == 0 or n == 1 for st, n in zip(to[:-1], t.shape)) and _dense_strides_ok(t)):
+            if any(st == 0 and n != 1 for st, n in zip(to[:-1], t.shape)):
+                return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            step = t.shape[-1]
+            for i in sorted(range(t.dim() - 1), key=t.stride):
+                to[i] = step
+                step = step * t.shape[i]
+        if max_pitch is None or t.shape[2] == 1 or to[2] < max_pitch:
+            return torch.empty_strided(t.shape, to, dtype=t.dtype, device=t.device)
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
@@ -1365,7 +1377,7 @@ def _linear_attn_check(q, k, v, log_decay, state, lengths=None):
 def _linear_attn_meta(q, k, v, log_decay, state, lengths, scale):
     _linear_attn_check(q, k, v, log_decay, state, lengths)
     B, H, _, D = q.shape
-    return _result_meta(q), torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
+    return _result_meta(q, _MAX_PITCH), torch.empty((B, H, D, D), dtype=torch.float32, device=q.device)
 
 
 def _linear_attn_bwd_meta(q, k, v, log_decay, state, lengths, d_out, d_state_out, scale, want_d_state):
@@ -1376,7 +1388,7 @@ def _linear_attn_bwd_meta(q, k, v, log_decay, state, lengths, d_out, d_state_out
     if d_state_out is not None and (tuple(d_state_out.shape) != (B, H, D, D) or d_state_out.dtype != torch.float32):
         raise ValueError("linear_attn_bwd: d_state_out must be float32 [B, H, D, D]")
     d_state = torch.empty((B, H, D, D) if want_d_state else (0,), dtype=torch.float32, device=q.device)
-    return _result_meta(q), _result_meta(k), _result_meta(v), d_state
+    return *(_result_meta(t, _MAX_PITCH) for t in (q, k, v)), d_state
 
 
 def _linear_attn_step_meta(q, k, v, log_decay, state, scale):
