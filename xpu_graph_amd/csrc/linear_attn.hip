@@ -33,7 +33,7 @@
 //
 // What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 270 others a chunk), of
 // which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 238 us (1.07 GB, 4.5 TB/s), B8 S2048
-// 122 us, B4 S2048 92 us (four segments: K and V twice, 0.40 GB), B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
+// 122 us, B4 S2048 98 us, B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
 // 580 us, B4 S2048 160 us (0.73 GB by the counters, 4.6 TB/s: seven tensors in where dv and dk share, nearly eight as it runs,
 // three out), B1 S32768 788 us.
 #include "sdpa_common.hpp"
@@ -711,8 +711,8 @@ __global__ __launch_bounds__(256) void group_sum_kernel(const GroupSum p) {
 }
 
 // One token: the state of a head is read, updated and written in place, and the row q S comes out of the same pass.
-// Bound by the state's bytes (two ways): B64 H32 D128 54 us, 268 MB, 5.0 TB/s; one sequence 3.5 us.  A workgroup takes 32 columns of one head's state: eight lanes per row (16 bytes each,
-// 128-byte lines), 32 rows at a time.
+// Bound by the state's bytes (two ways): B64 H32 D128 47 us, 268 MB, 5.7 TB/s on fresh states; one sequence 3.0 us.  A workgroup
+// takes W columns of one head's state, 16 bytes a lane, with streamed loads and stores (cached ones: 54 us).
 struct StepParams {
   const void* q;
   const void* k;
@@ -724,18 +724,19 @@ struct StepParams {
   int H, group;
   float scale;
 };
-template <typename T, int D>
+template <typename T, int D, int W>
 __global__ __launch_bounds__(256) void linear_attn_step_kernel(const StepParams p) {
-  __shared__ f32x4 red[4][8];
-  const int tid = threadIdx.x, c = (tid & 7) * 4, r0 = tid >> 3;
-  const int part = blockIdx.x % (D / 32), bh = blockIdx.x / (D / 32);
+  constexpr int LANES = W / 4, ROWS = 256 / LANES;  // lanes a row, rows at a time
+  __shared__ f32x4 red[4][LANES];
+  const int tid = threadIdx.x, l = tid % LANES, c = l * 4, r0 = tid / LANES;
+  const int part = blockIdx.x % (D / W), bh = blockIdx.x / (D / W);
   const int64_t b = bh / p.H;
   const int h = bh % p.H, hk = h / p.group;
-  const int col = 32 * part + c;
+  const int col = W * part + c;
   float* st = p.state + b * p.ss[0] + h * p.ss[1] + col;
-  f32x4 S[D / 32];
+  f32x4 S[D / ROWS];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) S[i] = *reinterpret_cast<const f32x4*>(st + (int64_t)(r0 + 32 * i) * D);
+  for (int i = 0; i < D / ROWS; ++i) S[i] = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(st + (int64_t)(r0 + ROWS * i) * D));
   const T* q = reinterpret_cast<const T*>(p.q) + b * p.qs[0] + h * p.qs[1];
   const T* k = reinterpret_cast<const T*>(p.k) + b * p.ks[0] + hk * p.ks[1];
   const T* v = reinterpret_cast<const T*>(p.v) + b * p.vs[0] + hk * p.vs[1] + col;
@@ -743,20 +744,22 @@ __global__ __launch_bounds__(256) void linear_attn_step_kernel(const StepParams 
   f32x4 vv, acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int r = 0; r < 4; ++r) vv[r] = to_f32(v[r]);
+  float kr[D / ROWS], qr[D / ROWS];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    const float kr = to_f32(k[r0 + 32 * i]), qr = to_f32(q[r0 + 32 * i]);
-    S[i] = S[i] * lam + kr * vv;
-    *reinterpret_cast<f32x4*>(st + (int64_t)(r0 + 32 * i) * D) = S[i];
-    acc += qr * S[i];
+  for (int i = 0; i < D / ROWS; ++i) kr[i] = to_f32(k[r0 + ROWS * i]), qr[i] = to_f32(q[r0 + ROWS * i]);
+#pragma unroll
+  for (int i = 0; i < D / ROWS; ++i) {
+    S[i] = S[i] * lam + kr[i] * vv;
+    __builtin_nontemporal_store(S[i], reinterpret_cast<f32x4*>(st + (int64_t)(r0 + ROWS * i) * D));
+    acc += qr[i] * S[i];
   }
 #pragma unroll
-  for (int off = 8; off < 64; off <<= 1)
+  for (int off = LANES; off < 64; off <<= 1)
 #pragma unroll
     for (int r = 0; r < 4; ++r) acc[r] += __shfl_xor(acc[r], off, kWave);
-  if ((tid & 63) < 8) red[tid >> 6][tid & 7] = acc;
+  if ((tid & 63) < LANES) red[tid >> 6][l] = acc;
   __syncthreads();
-  if (tid < 8) {
+  if (tid < LANES) {
     f32x4 t = red[0][tid];
 #pragma unroll
     for (int i = 1; i < 4; ++i) t += red[i][tid];
@@ -772,14 +775,14 @@ constexpr int64_t kMaxPitch = 1 << 26;  // elements between tokens: 32 rows stay
 int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
 
 // How many segments the tokens of a head are cut into, four chunks at least each.  Cutting reads K and V twice; not cutting leaves
-// the chip idle where there are few heads, each of which takes 1.4 us a chunk.  Up to half the heads that fill it with one wave a
-// SIMD they are cut to fill it once, or twice where that would be less than four segments.  Measured (bf16 D 128, us, uncut /
-// segments: once, twice the chip): forward 32 heads S 32768 1362 / 8: 336, 16: 356; 64 heads S 8192 339 / 4: 179, 8: 182; 96 heads
-// S 4096 174 / 2: 147, 5: 129; 128 heads S 2048 99 / 2: 96, 4: 92; 192 heads S 2048 109 / 2: 132, 3: 145; backward (three times the
-// heads) 32 heads S 32768 1242 / 2: 1007, 5: 790, 64 heads S 8192 348 / 2: 398.
+// the chip idle where there are few heads, each of which takes 1.4 us a chunk.  With fewer than half the heads that fill it with
+// one wave a SIMD they are cut to fill it once, or twice where that would be less than four segments.  Measured (bf16 D 128, us,
+// uncut / segments: once, twice the chip): forward 32 heads S 32768 1362 / 8: 336, 16: 356; 64 heads S 8192 348 / 4: 181, 8: 180; 96
+// heads S 4096 176 / 2: 154, 5: 137; 128 heads S 2048 98 / 2: 98, 4: 102; 192 heads 109 / 2: 132; backward (three times the heads)
+// 32 heads S 32768 1242 / 2: 1007, 5: 790, 64 heads S 8192 358 / 4: 394.
 void segments(int64_t heads, int64_t n_problems, int64_t S, int64_t D, int& n_seg, int& seg_chunks) {
   const int64_t chunks = chunks_of(S), groups = heads * n_problems, full = 256 * (128 / D);
-  int64_t n = groups > full / 2 ? 1 : (full / groups >= 4 ? full : 2 * full) / groups;
+  int64_t n = groups >= full / 2 ? 1 : (full / groups >= 4 ? full : 2 * full) / groups;
   if (n > chunks / 4) n = chunks / 4;
   if (n < 1) n = 1;
   seg_chunks = (int)((chunks + n - 1) / n);
@@ -1031,18 +1034,24 @@ extern "C" int xg_linear_attn_step(const void* q, const void* k, const void* v, 
   p.H = (int)H;
   p.group = (int)(H / Hkv);
   p.scale = scale;
-  const dim3 grid((unsigned)(B * H * (D / 32)));
+  // 64 columns a workgroup (B64 H32 D128 47 us; 32: 49, 128: 49), 32 where those are too few to give every compute unit one
+  // (B1 H32 3.5 us with 64, 3.0 with 32; B8 H32 7.5 and 7.9)
+  const bool wide = B * H * (D / 64) >= 256;
+  const dim3 grid((unsigned)(B * H * (D / (wide ? 64 : 32))));
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == XG_BF16) {
-    if (D == 64)
-      hipLaunchKernelGGL((linear_attn_step_kernel<bf16_t, 64>), grid, dim3(256), 0, st, p);
+  auto go = [&](auto type, auto dim) {
+    typedef decltype(type) T;
+    constexpr int DIM = decltype(dim)::value;
+    if (wide)
+      hipLaunchKernelGGL((linear_attn_step_kernel<T, DIM, 64>), grid, dim3(256), 0, st, p);
     else
-      hipLaunchKernelGGL((linear_attn_step_kernel<bf16_t, 128>), grid, dim3(256), 0, st, p);
-  } else {
-    if (D == 64)
-      hipLaunchKernelGGL((linear_attn_step_kernel<f16_t, 64>), grid, dim3(256), 0, st, p);
-    else
-      hipLaunchKernelGGL((linear_attn_step_kernel<f16_t, 128>), grid, dim3(256), 0, st, p);
-  }
+      hipLaunchKernelGGL((linear_attn_step_kernel<T, DIM, 32>), grid, dim3(256), 0, st, p);
+  };
+  const std::integral_constant<int, 64> d64;
+  const std::integral_constant<int, 128> d128;
+  if (dtype == XG_BF16)
+    D == 64 ? go(bf16_t{}, d64) : go(bf16_t{}, d128);
+  else
+    D == 64 ? go(f16_t{}, d64) : go(f16_t{}, d128);
   return status_from_hip(hipGetLastError());
 }
