@@ -193,6 +193,23 @@ def test_a_batch_of_many_heads_takes_the_grouped_path(device):
     check_qk(device, torch.bfloat16, CASES[1], 2, 30, 7, 4001, "own", packed=True)  # four heads a thread, a group that ends early
 
 
+@pytest.mark.parametrize("case,S", [(CASES[1], 3001), (CASES[4], 2001), (CASES[6], 2001), (CASES[6], 6001)])
+def test_two_and_four_heads_a_thread(device, case, S):
+    check_qk(device, torch.bfloat16, case, 2, 9, 3, S, "own")  # (groups of the last odd head)
+
+
+@pytest.mark.parametrize("case,S", [(CASES[6], 1501), (CASES[6], 6001), (CASES[4], 6001), (CASES[2], 9001)])
+def test_two_and_eight_heads_a_thread(device, case, S):
+    D, R, sections, woven, kind, per, _ = case
+    B, H, P = 2, 11, 70
+    x = make(B, H + 2, S, D, torch.float16, device, 5)[:, 1:-1]  # a part of something else
+    cos, sin = tables(P if kind != "none" else S, R // 2, device, torch.float32, 2, per == 2)
+    pos = make_positions(kind if kind != "s" else "bs", max(len(sections), 1), B, S, P, device, 3)
+    ang = angles(cos, sin, pos, sections, woven, B, S, R)
+    assert_rounded_once(_ops().rope_axes(x, cos, sin, pos, sections, woven), *turn(x.double(), ang, R), "rope_axes")
+    assert_rounded_once(_ops().rope_axes_bwd(x, cos, sin, pos, sections, woven), *turn_back(x.double(), ang, R), "rope_axes_bwd")
+
+
 def test_extreme_rows(device):
     """A row of zeros normalises to zeros; the largest and the smallest values of the type do not overflow in fp32."""
     D, eps = 64, 1e-6

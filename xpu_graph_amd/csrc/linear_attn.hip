@@ -34,8 +34,8 @@
 // What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 270 others a chunk), of
 // which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 238 us (1.07 GB, 4.5 TB/s), B8 S2048
 // 122 us, B4 S2048 98 us, B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
-// 580 us, B4 S2048 160 us (0.73 GB by the counters, 4.6 TB/s: seven tensors in where dv and dk share, nearly eight as it runs,
-// three out), B1 S32768 788 us.
+// 580 us, B4 S2048 160 us (0.67 GB by the counters: dv and dk share all they can; 384 workgroups on 256 compute units), B1 S32768
+// 788 us.
 #include "sdpa_common.hpp"
 
 namespace xg {

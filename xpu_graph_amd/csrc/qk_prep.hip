@@ -16,9 +16,11 @@
 // takes D/16 lanes (rounded up to a power of two for the row sums, which stay inside the wavefront), and a thread
 // takes kHeads heads of one token, which share the table row.  Queries and keys go out in one launch.  All sums and
 // the rotation are fp32; one rounding per output.
-// Measured (bf16, D 128): rope_axes B2 S6144 H32, three axes 36 us, 201 MB, 5.6 TB/s; qk_norm_rope B4 S2048 H32/8 34 us, 168 MB,
-// 4.9 TB/s, H32/32 51 us, 268 MB, 5.3 TB/s, its backward 78 + 4 us, 403 MB, 5.0 TB/s.  D 96 leaves two of a row's eight lanes
-// idle: fp16 B3 S1371 H10/5 13 us forward, 18 + 4 us backward.
+// Measured on fresh inputs (bf16, D 128): rope_axes B2 S6144 H32, three axes 39 us, 201 MB, 5.1 TB/s; qk_norm_rope B4 S2048 H32/8
+// 32 us, 168 MB, 5.2 TB/s, H32/32 51 us, 268 MB, 5.3 TB/s, its backward with the sum of the weight gradients 78 us, 403 MB, 5.1 TB/s
+// (a copy of that size: 6.3).  Loads behind a condition each cost a quarter (47, 45, 72, 93 us), cached loads and results that
+// lie head by head where the inputs lie token by token a tenth more.  D 96 leaves two of a row's eight lanes idle: fp16 B3 S1371
+// H10/5 13 us forward, 18 + 4 us backward.
 #include "xg_common.hpp"
 
 namespace xg {
@@ -487,20 +489,23 @@ int run_prep(Prep& p, int64_t tokens, int dtype, hipStream_t stream) {
     if (dtype == XG_F16) return launch_prep<f16_t, NORM, FULL, kHeads>(p, tokens, stream);
     return launch_prep<float, NORM, FULL, kHeads>(p, tokens, stream);
   };
-  // Several heads a thread share one read of the tables (8 without the norm, 4 with it, whose weights and sums take
-  // registers); few rows are spread over as many threads as there are.
+  // Several heads a thread share one read of the tables and keep more bytes on their way; few rows are spread over as many
+  // threads as there are.  By the threads that one head each would make, bf16 D 128 on fresh inputs, us with one / two / four
+  // (eight) heads a thread: rope_axes, three axes, H32 131 k (S 512) 5.4 / 5.5 / 6.9 (9.0), 524 k 12.4 / 8.9 / 9.1 (10.5), 1.05 M
+  // 20.4 / 17.4 / 14.2 (14.5), 3.1 M - (39); qk_norm_rope H32/8 328 k (S 1024) 6.6 / 6.9 / 8.0, 655 k 11.7 / 9.5 / 10.3, 1.3 M
+  // 19.7 / 18.2 / 16.1, 2.6 M 32 with four, 38 with eight (registers).
   const int64_t threads = (tokens * (p.side[0].H + p.side[1].H)) << p.tpr_log2;
+  auto with = [&](auto heads) { return p.half_off ? go(std::true_type{}, heads) : go(std::false_type{}, heads); };
   constexpr int kMany = NORM ? 4 : 8;
-  const std::integral_constant<int, kMany> many;
-  const std::integral_constant<int, 1> one;
-  if (threads >= 4 * 256 * 1024) return p.half_off ? go(std::true_type{}, many) : go(std::false_type{}, many);
-  return p.half_off ? go(std::true_type{}, one) : go(std::false_type{}, one);
+  if (threads >= 4 * 256 * 1024) return with(std::integral_constant<int, kMany>{});
+  if (threads >= 256 * 1024) return with(std::integral_constant<int, 2>{});
+  return with(std::integral_constant<int, 1>{});
 }
 
 constexpr int kBwdHeads = 2;
 
 // Blocks of the two sides of the backward, in proportion to the rows: as many as the chip holds at once (three per compute
-// unit by registers; B4 S2048 H32/32 D128 bf16: 80.7 us with 768, 84 with 1536, 101 with 1024, 4.99 TB/s).
+// unit by registers; B4 S2048 H32/32 D128 bf16 on one set of inputs: 80.7 us with 768, 84 with 1536, 101 with 1024).
 void bwd_blocks(int64_t tokens, int64_t H0, int64_t H1, int64_t D, int& n0, int& n1) {
   int log2 = 0;
   while ((1 << log2) < D / 16) ++log2;
