@@ -154,7 +154,7 @@ def test_without_states(device, dtype, D, state, d_state):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("B,H,Hkv,S,D", [(1, 6, 2, 70, 64), (2, 8, 1, 333, 128), (1, 12, 4, 129, 128), (3, 2, 1, 1, 64), (4, 4, 2, 333, 64), (2, 16, 4, 70, 128)])
+@pytest.mark.parametrize("B,H,Hkv,S,D", [(1, 6, 2, 70, 64), (2, 8, 1, 333, 128), (1, 12, 4, 129, 128), (3, 2, 1, 1, 64), (4, 4, 2, 333, 64), (2, 16, 4, 70, 128), (2, 16, 4, 700, 128)])
 def test_shared_heads(device, dtype, B, H, Hkv, S, D):
     run_all(device, dtype, B, H, Hkv, S, D)
 
@@ -544,3 +544,24 @@ def test_gradients_that_do_not_exist_are_refused(device):
         s1 = torch.zeros(1, 2, 64, 64, device=device)
         y = x.clone()
         assert torch.equal(_ops().linear_attn_step(y, y, y, g, s1, 0.1), _ops().linear_attn_step(x, x, x, g, torch.zeros_like(s1), 0.1))
+
+
+def test_calls_that_overlap_on_two_streams(device):
+    """Workspaces, partial sums and states of one call are not those of another."""
+    g = decays(4, device)
+    sets = [[make((2, h, 900, 128), torch.bfloat16, device, 10 * i + j) for j, h in enumerate((4, 2, 2, 4))] for i in range(2)]
+
+    def f(q, k, v, go):
+        o, s = _ops().linear_attn(q, k, v, g, None, None, 0.1)
+        return (o, s, *_ops().linear_attn_bwd(q, k, v, g, None, None, go, s, 0.1, True))
+
+    want = [f(*x) for x in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in sets], [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(f(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for run in got[i] for a, b in zip(want[i], run))

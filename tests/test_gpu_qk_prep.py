@@ -238,6 +238,22 @@ def test_a_position_outside_the_tables_gives_nan_and_touches_nothing_else(device
     assert torch.isnan(got[:, :, hurt]).all() and torch.equal(got[:, :, ~hurt], want[:, :, ~hurt])
 
 
+@pytest.mark.parametrize("per_element", [False, True])
+def test_a_position_outside_one_axis_gives_nan_in_its_row(device, per_element):
+    x, g = make(1, 2, 5, 64, torch.bfloat16, device, 1), make(1, 2, 5, 64, torch.bfloat16, device, 2)
+    cos, sin = tables(10, 16, device, torch.float32, 2, per_element)
+    good = torch.tensor([0, 1, 2, 3, 9], device=device)
+    bad = torch.tensor([0, 10, 2, -(2**40), 9], device=device)
+    want, got = (_ops().rope_axes(x, cos, sin, p, [16]) for p in (good, bad))
+    out = torch.tensor([1, 3], device=device)
+    assert torch.isnan(got[:, :, out, :32]).all() and torch.equal(got[:, :, out, 32:], x[:, :, out, 32:])
+    kept = torch.tensor([0, 2, 4], device=device)
+    assert torch.equal(got[:, :, kept], want[:, :, kept])
+    args = lambda p: (x, x, None, None, g, g, cos, sin, p, [16], False, 1e-6, False)  # noqa: E731
+    want, got = (_ops().qk_norm_rope_bwd(*args(p))[0] for p in (good, bad))
+    assert torch.isnan(got[:, :, out]).all() and torch.equal(got[:, :, kept], want[:, :, kept])
+
+
 @pytest.mark.parametrize("D", [64, 96, 128])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_agrees_with_the_norm_and_the_rotation_in_sequence(device, D, dtype):
