@@ -565,3 +565,53 @@ def test_calls_that_overlap_on_two_streams(device):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for run in got[i] for a, b in zip(want[i], run))
+
+
+def entry(name, *args):
+    """A C entry point on the current stream; tensors by their addresses, tuples as strides."""
+    import ctypes
+
+    lib = _xops()._lib.lib()
+    raw = [a.data_ptr() if isinstance(a, torch.Tensor) else (ctypes.c_int64 * len(a))(*a) if isinstance(a, tuple) else a for a in args]
+    return getattr(lib, name)(*raw, torch.cuda.current_stream().cuda_stream)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("given", [True, False])
+def test_entry_points_without_tokens_carry_the_state(device, D, given):
+    """S = 0: the state after the last token is the one before the first, the gradient of the initial state that of the final one."""
+    B, H, Hkv = 3, 4, 2
+    before = torch.randn(B, H, D, D, device=device) if given else None
+    want = before if given else torch.zeros(B, H, D, D, device=device)
+    st = (0, 0, 0)
+
+    def fwd(out):
+        return entry("xg_linear_attn", None, None, None, None, before, None, 0, None, out, None, 0, B, H, Hkv, 0, D, st, st, st, st, 1.0, 2)
+
+    def bwd(out):
+        return entry("xg_linear_attn_bwd", *[None] * 6, 0, None, before, None, None, None, out, None, 0, B, H, Hkv, 0, D, *[st] * 7, 1.0, 2)
+
+    for call in (fwd, bwd):
+        out = torch.full((B, H, D, D), 7.0, device=device)
+        assert call(out) == 0 and torch.equal(out, want)
+        assert call(None) == 0
+        if given:  # in place
+            assert call(before) == 0 and torch.equal(before, want)
+        off = torch.full((B * H * D * D + 1,), 7.0, device=device)[1:]
+        assert call(off) == -3 and (off == 7).all()
+
+
+def test_an_empty_prompt_piece_recorded_in_a_graph(device):
+    B, H, D = 2, 3, 64
+    s0, out, st = torch.randn(B, H, D, D, device=device), torch.zeros(B, H, D, D, device=device), (0, 0, 0)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        rc = entry("xg_linear_attn", None, None, None, None, s0, None, 0, None, out, None, 0, B, H, H, 0, D, st, st, st, st, 1.0, 2)
+    assert rc == 0
+    for _ in range(3):
+        s0.normal_()
+        out.zero_()
+        graph.replay()
+        assert torch.equal(out, s0)

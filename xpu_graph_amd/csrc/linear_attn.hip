@@ -769,6 +769,11 @@ __global__ __launch_bounds__(256) void linear_attn_step_kernel(const StepParams 
   }
 }
 
+// No tokens: the state before them is the state after them (zeros where there is none).
+__global__ __launch_bounds__(256) void carry_state_kernel(const f32x4* __restrict__ from, f32x4* __restrict__ to, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from ? from[i] : f32x4{0.f, 0.f, 0.f, 0.f};
+}
+
 // ------------------------------------------------------------------ host side
 constexpr int64_t kMaxPitch = 1 << 26;  // elements between tokens: 32 rows stay inside 32-bit offsets
 
@@ -823,6 +828,27 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
   return fill(o.s, s);
 }
 
+// Whether a kernel could reach p: not where there is no device, nor in host memory that HIP does not know.
+bool on_gpu(const void* p) {
+  hipPointerAttribute_t at;
+  const hipError_t e = hipPointerGetAttributes(&at, p);
+  if (e == hipSuccess) return at.type != hipMemoryTypeUnregistered;
+  (void)hipGetLastError();  // (it would be taken for the next launch's)
+  return e != hipErrorNoDevice;
+}
+
+// The state results of a call without tokens.  Such a call refuses no pointer, as it reads nothing through q, k and v; so what it
+// does read and write is looked at first, and left alone where no kernel could reach it.
+int carry_state(const float* from, float* to, int64_t heads, int64_t D, hipStream_t st) {
+  if (!to || from == to) return XG_OK;
+  if (!aligned_to(to, 16) || (from && !aligned_to(from, 16))) return XG_ERR_BAD_ALIGN;
+  if (!on_gpu(to) || (from && !on_gpu(from))) return XG_OK;
+  const int64_t n = heads * D * D / 4, blocks = (n + 255) / 256;
+  hipLaunchKernelGGL(carry_state_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, reinterpret_cast<const f32x4*>(from),
+                     reinterpret_cast<f32x4*>(to), n);
+  return status_from_hip(hipGetLastError());
+}
+
 template <typename T, int D>
 int launch(const Params& p, int n_problems, hipStream_t st) {
   const dim3 grid((unsigned)(p.B * p.H * p.n_seg), (unsigned)n_problems), all(grid.x * grid.y), block(D * 2);
@@ -856,7 +882,8 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
   using namespace xg;
   using namespace xg::linattn;
   if (int rc = check(B, H, Hkv, S, D, scale, dtype)) return rc;
-  if (B == 0 || H == 0 || S == 0) return XG_OK;
+  if (B == 0 || H == 0) return XG_OK;
+  if (S == 0) return carry_state(state, state_out, B * H, D, reinterpret_cast<hipStream_t>(stream));
   if (!log_decay || !out) return XG_ERR_NULL_PTR;
   if (!aligned_to(out, 16) || !aligned_to(log_decay, 4) || (state && !aligned_to(state, 16)) || (state_out && !aligned_to(state_out, 16)) ||
       (workspace && !aligned_to(workspace, 16)) || (lengths && !aligned_to(lengths, lengths_64bit ? 8 : 4)))
@@ -904,7 +931,8 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   using namespace xg;
   using namespace xg::linattn;
   if (int rc = check(B, H, Hkv, S, D, scale, dtype)) return rc;
-  if (B == 0 || H == 0 || S == 0) return XG_OK;
+  if (B == 0 || H == 0) return XG_OK;
+  if (S == 0) return carry_state(d_state_out, d_state, B * H, D, reinterpret_cast<hipStream_t>(stream));
   if (!log_decay || !dq || !dk || !dv) return XG_ERR_NULL_PTR;
   for (const void* t : {(const void*)dq, (const void*)dk, (const void*)dv, (const void*)state, (const void*)d_state_out, (const void*)d_state,
                         (const void*)workspace})
