@@ -525,7 +525,8 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  * xg_linear_attn_bwd: dq, dk, dv (own strides, as the gradients of xg_sdpa)
  *   and d_state (NULL: not wanted) from d_out and d_state_out (NULL: none).
  *   log_decay gets no gradient.  Sums in a fixed order, no atomics; the
- *   gradients of shared heads are added up in fp32.  workspace:
+ *   gradients of shared heads are added up in fp32 (H = 0: dk and dv of the
+ *   key heads are zeros).  workspace:
  *   xg_linear_attn_bwd_workspace_floats fp32.
  * xg_linear_attn_step: one token; `state` is updated in place.  q, k, v, out:
  *   strides of batch and head, any alignment; state_strides: batch and head,

@@ -615,3 +615,32 @@ def test_an_empty_prompt_piece_recorded_in_a_graph(device):
         out.zero_()
         graph.replay()
         assert torch.equal(out, s0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_key_heads_without_query_heads_get_zero_gradients(device, dtype):
+    """A gradient of a key head is a sum over its query heads; over none it is zero."""
+    B, Hkv, S, D = 2, 3, 37, 64
+    q, g = torch.empty(B, 0, S, D, device=device, dtype=dtype), torch.empty(0, device=device)
+    heads = make((B, 2 * Hkv, S, D), dtype, device, 1)
+    k, v = heads[:, :Hkv], heads[:, Hkv:]
+    s0 = torch.empty(B, 0, D, D, device=device)
+    for _ in range(2):
+        del_me = [torch.full_like(k, 7.0) for _ in range(4)]  # what the allocator hands out next is not zero
+        del del_me
+        o, s = _ops().linear_attn(q, k, v, g, s0, None, 1.0)
+        dq, dk, dv, d0 = _ops().linear_attn_bwd(q, k, v, g, s0, None, q, s0, 1.0, True)
+        assert o.shape == dq.shape == q.shape and s.shape == d0.shape == s0.shape
+        assert dk.shape == dv.shape == k.shape and (dk == 0).all() and (dv == 0).all()
+    # the entry point writes the rows of its operands and nothing between them
+    dk, dv = (torch.full((B, S, Hkv + 1, D), 7.0, device=device, dtype=dtype).transpose(1, 2) for _ in range(2))
+    st, code = tuple(dk.stride()[:3]), 2 if dtype == torch.bfloat16 else 1
+    n = (0, 0, 0)
+
+    def bwd(dk, dv, Hkv=Hkv):
+        return entry("xg_linear_attn_bwd", *[None] * 6, 0, None, None, None, dk, dv, None, None, 0, B, 0, Hkv, S, D, *[n] * 5, st, st, 1.0, code)
+
+    assert bwd(dk, None) == -4 and bwd(dk, None, Hkv=0) == 0 and (dk == 7).all()
+    assert bwd(dk, dv) == 0
+    for x in (dk, dv):
+        assert (x[:, :Hkv] == 0).all() and (x[:, Hkv:] == 7).all()

@@ -105,3 +105,21 @@ def test_entry_points_refuse_before_any_launch():
 
     assert step(B=0) == 0 and step(state=None) == -4 and step(D=32) == -2 and step(state=off) == -3 and step(ss=(8192, 4098)) == -3
     assert step(ss=(0, 4096)) == -2 and step(ss=(8192, 0)) == -2 and step(ss=(4096, 4096)) == -2  # states that overlap
+
+
+def test_key_heads_without_query_heads():
+    q, k = meta(2, 0, 8, 64), meta(2, 3, 8, 64)
+    dq, dk, dv, _ = OPS.linear_attn_bwd(q, k, k, meta(0, dtype=torch.float32), None, None, q, None, 1.0, False)
+    assert dq.shape == q.shape and dk.shape == dv.shape == k.shape
+    lib = _lib.lib()
+    buf = ctypes.create_string_buffer(1 << 12)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 15) & ~15)
+    off = ctypes.c_void_p(p.value + 8)
+    st = (ctypes.c_int64 * 3)(1 << 14, 1 << 12, 64)
+
+    def bwd(dk=p, dv=p, B=2, Hkv=3, S=8, D=64, s=st):
+        return lib.xg_linear_attn_bwd(*[None] * 6, 0, None, None, None, dk, dv, p, None, 0, B, 0, Hkv, S, D, *[st] * 5, s, s, 1.0, 2, None)
+
+    assert bwd(B=0) == 0 and bwd(S=0) == 0 and bwd(Hkv=0) == 0  # nothing to write
+    assert bwd(dk=None) == -4 and bwd(dv=None) == -4 and bwd(dk=off) == -3 and bwd(s=None) == -4
+    assert bwd(D=96) == -2 and bwd(Hkv=1 << 40) == -5 and bwd(s=(ctypes.c_int64 * 3)(1, 2, 3)) == -3

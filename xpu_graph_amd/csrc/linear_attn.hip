@@ -700,7 +700,8 @@ __global__ __launch_bounds__(256) void group_sum_kernel(const GroupSum p) {
   const int hk = (int)((row / p.S) % p.Hkv);
   const int64_t b = row / ((int64_t)p.S * p.Hkv);
   const float* src = p.part[blockIdx.y] + (((b * p.Hkv + hk) * p.group) * p.S + s) * (int64_t)p.D + c;
-  f32x4 a = *reinterpret_cast<const f32x4*>(src);
+  f32x4 a = {0.f, 0.f, 0.f, 0.f};  // (no query heads at all)
+  if (p.group) a = *reinterpret_cast<const f32x4*>(src);
   for (int g = 1; g < p.group; ++g) a += *reinterpret_cast<const f32x4*>(src + (int64_t)g * p.S * p.D);
   typedef T T4 __attribute__((ext_vector_type(4)));
   T4 y;
@@ -840,7 +841,7 @@ bool on_gpu(const void* p) {
 // The state results of a call without tokens.  Such a call refuses no pointer, as it reads nothing through q, k and v; so what it
 // does read and write is looked at first, and left alone where no kernel could reach it.
 int carry_state(const float* from, float* to, int64_t heads, int64_t D, hipStream_t st) {
-  if (!to || from == to) return XG_OK;
+  if (!to || from == to || heads == 0) return XG_OK;
   if (!aligned_to(to, 16) || (from && !aligned_to(from, 16))) return XG_ERR_BAD_ALIGN;
   if (!on_gpu(to) || (from && !on_gpu(from))) return XG_OK;
   const int64_t n = heads * D * D / 4, blocks = (n + 255) / 256;
@@ -858,6 +859,16 @@ int launch(const Params& p, int n_problems, hipStream_t st) {
     hipLaunchKernelGGL((scan_states_kernel<D>), dim3((unsigned)(p.B * p.H * (D * D / 1024)), sums), dim3(256), 0, st, p);
   }
   hipLaunchKernelGGL((linear_attn_kernel<T, D>), all, block, 0, st, p);
+  return status_from_hip(hipGetLastError());
+}
+
+int sum_groups(const GroupSum& p, int dtype, hipStream_t st) {
+  if (p.n > 0xffffff00LL) return XG_ERR_TOO_LARGE;  // threads of a launch
+  const dim3 grid((unsigned)((p.n + 255) / 256), 2);
+  if (dtype == XG_BF16)
+    hipLaunchKernelGGL((group_sum_kernel<bf16_t>), grid, dim3(256), 0, st, p);
+  else
+    hipLaunchKernelGGL((group_sum_kernel<f16_t>), grid, dim3(256), 0, st, p);
   return status_from_hip(hipGetLastError());
 }
 
@@ -931,8 +942,24 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
   using namespace xg;
   using namespace xg::linattn;
   if (int rc = check(B, H, Hkv, S, D, scale, dtype)) return rc;
-  if (B == 0 || H == 0) return XG_OK;
+  if (B == 0) return XG_OK;
   if (S == 0) return carry_state(d_state_out, d_state, B * H, D, reinterpret_cast<hipStream_t>(stream));
+  GroupSum gs{};
+  gs.n = B * Hkv * S * D / 4;
+  gs.Hkv = (int)Hkv;
+  gs.S = (int)S;
+  gs.D = (int)D;
+  if (H == 0) {  // sums over no query heads
+    if (Hkv == 0) return XG_OK;
+    if (Hkv > (1 << 24) || B * Hkv > (1 << 20)) return XG_ERR_TOO_LARGE;  // (as check() for the query heads)
+    gs.out[0] = dv;
+    gs.out[1] = dk;
+    if (!dk || !dv) return XG_ERR_NULL_PTR;
+    if (!aligned_to(dk, 16) || !aligned_to(dv, 16)) return XG_ERR_BAD_ALIGN;
+    if (int rc = fill(gs.os[0], dv_strides)) return rc;
+    if (int rc = fill(gs.os[1], dk_strides)) return rc;
+    return sum_groups(gs, dtype, reinterpret_cast<hipStream_t>(stream));
+  }
   if (!log_decay || !dq || !dk || !dv) return XG_ERR_NULL_PTR;
   for (const void* t : {(const void*)dq, (const void*)dk, (const void*)dv, (const void*)state, (const void*)d_state_out, (const void*)d_state,
                         (const void*)workspace})
@@ -995,7 +1022,6 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
     r->s_inter = 1.f;
   }
   for (int i = 0; i < 3; ++i) p.pr[i].seg_states = workspace + i * seg_floats;
-  GroupSum gs{};
   if (group > 1) {
     for (int i = 0; i < 2; ++i) {
       Problem& r = p.pr[i];
@@ -1008,23 +1034,12 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
       r.os[2] = D;
       r.out_f32 = 1;
     }
-    gs.n = B * Hkv * S * D / 4;
-    gs.Hkv = (int)Hkv;
-    gs.S = (int)S;
-    gs.D = (int)D;
     gs.group = group;
-    if (gs.n > 0xffffff00LL) return XG_ERR_TOO_LARGE;  // threads of a launch
+    if (gs.n > 0xffffff00LL) return XG_ERR_TOO_LARGE;  // (before any launch)
   }
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   if (int rc = launch_any(p, 3, D, dtype, st)) return rc;
-  if (group > 1) {
-    const dim3 grid((unsigned)((gs.n + 255) / 256), 2);
-    if (dtype == XG_BF16)
-      hipLaunchKernelGGL((group_sum_kernel<bf16_t>), grid, dim3(256), 0, st, gs);
-    else
-      hipLaunchKernelGGL((group_sum_kernel<f16_t>), grid, dim3(256), 0, st, gs);
-  }
-  return status_from_hip(hipGetLastError());
+  return group > 1 ? sum_groups(gs, dtype, st) : XG_OK;
 }
 
 extern "C" int xg_linear_attn_step(const void* q, const void* k, const void* v, const float* log_decay, float* state, void* out, int64_t B,

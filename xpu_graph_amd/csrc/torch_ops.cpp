@@ -370,7 +370,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> linear_attn_bwd(const Tensor& q_in, c
   Tensor d_state = want_d_state ? at::empty({B, H, D, D}, fp32) : at::empty({0}, fp32);
   if (dq.numel() == 0) {
     if (want_d_state) has(d_state_out_in) ? d_state.copy_(*d_state_out_in) : d_state.zero_();
-    return {dq, dk, dv, d_state};
+    return {dq, dk.zero_(), dv.zero_(), d_state};  // (key heads without query heads: sums of nothing)
   }
   const Tensor q = token_operand(q_in), k = token_operand(k_in), v = token_operand(v_in), d_out = token_operand(d_out_in), g = log_decay_in.contiguous();
   const OptTensor state = state_operand(state_in), d_state_out = state_operand(d_state_out_in), lengths = contiguous(lengths_in);
