@@ -465,7 +465,7 @@ int xg_rope(const void* x, const void* cos_table, const void* sin_table, void* o
  *     once, where xg_rms_norm followed by xg_rope rounds twice.
  *   xg_qk_norm_rope_bwd: dq, dk from the upstream gradients gq, gk of the two
  *     outputs, and gw_q, gw_k [D] (in w_dtype; NULL: not wanted), summed over
- *     rows in a fixed order (no atomics) through a workspace of
+ *     rows (zeros over none) in a fixed order (no atomics) through a workspace of
  *     xg_qk_norm_rope_bwd_workspace_floats fp32 (NULL when neither is wanted).
  * No counterpart in the reference: what it leaves to eager before
  *   aten.scaled_dot_product_attention

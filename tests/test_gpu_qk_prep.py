@@ -474,3 +474,29 @@ def test_results_lie_as_the_shape_functions_say(device, layout):
     lin = lambda x, g: _ops().linear_attn(x, x, x, g, None, None, 1.0)  # noqa: E731
     g = torch.zeros(x.shape[1], device=device)
     assert [t.stride() for t in lin(x, g)] == [t.stride() for t in lin(as_meta(x), as_meta(g))]
+
+
+@pytest.mark.parametrize("w_dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Hkv,S", [(0, 2, 1, 5), (2, 2, 1, 0), (2, 0, 0, 5)])
+def test_the_entry_point_sums_weight_gradients_over_no_rows(device, w_dtype, B, H, Hkv, S):
+    """Weight gradients are sums over rows; over none they are zero, and written."""
+    import ctypes
+
+    lib = _xops()._lib.lib()
+    D = 64
+    cos, sin = tables(8, D // 2, device, torch.float32, 1, False)
+    r = _xops()._lib.XgRotary(cos.data_ptr(), sin.data_ptr(), 8, D // 2, D // 2, D)
+    r.axes, r.table_dtype = 1, 0
+    dtype = torch.bfloat16 if w_dtype == torch.float32 else w_dtype
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    st = (ctypes.c_int64 * 3)(0, 0, 0)
+    assert lib.xg_qk_norm_rope_bwd_workspace_floats(B, H, Hkv, S, D) == 0
+    both = [torch.full((D,), 7.0, device=device, dtype=w_dtype) for _ in range(2)]
+    for gws in (both, (both[0], None), (None, None)):
+        for x in both:
+            x.fill_(7.0)
+        p = [x.data_ptr() if x is not None else None for x in gws]
+        rc = lib.xg_qk_norm_rope_bwd(*[None] * 8, *p, None, 0, B, H, Hkv, S, D, *[st] * 6, r, 1e-6, code[dtype], code[w_dtype], torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+        for x, wanted in zip(both, gws):
+            assert (x == (0 if wanted is not None else 7)).all()

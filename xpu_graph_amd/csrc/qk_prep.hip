@@ -367,7 +367,7 @@ __global__ __launch_bounds__(1024) void gw_sum_kernel(const float* __restrict__ 
   const int c = threadIdx.x & 15, l = threadIdx.x >> 4;
   const int col = blockIdx.x * 16 + c;
   const int rows = second ? blocks1 : blocks0;
-  const float* src = part + (second ? (int64_t)blocks0 * D : 0) + col;
+  const float* src = part + (second ? (int64_t)blocks0 * D : 0) + col;  // (not read where there are no rows)
   float a = 0.f;
 #pragma unroll 8
   for (int r = l; r < rows; r += 64) a += src[(int64_t)r * D];
@@ -521,6 +521,22 @@ void bwd_blocks(int64_t tokens, int64_t H0, int64_t H1, int64_t D, int& n0, int&
   n1 = (int)count(H1);
 }
 
+// The weight gradients from the blocks' rows (zeros over none).
+int sum_weight_grads(const float* part, int n0, int n1, int64_t D, void* gw_q, void* gw_k, int w_dtype, hipStream_t st) {
+  const dim3 grid((unsigned)(D / 16), 2);
+  auto sum = [&](auto zero) {
+    typedef decltype(zero) WT;
+    hipLaunchKernelGGL((gw_sum_kernel<WT>), grid, dim3(1024), 0, st, part, n0, n1, (int)D, (WT*)gw_q, (WT*)gw_k);
+  };
+  if (w_dtype == XG_F32)
+    sum(0.f);
+  else if (w_dtype == XG_BF16)
+    sum((bf16_t)0.f);
+  else
+    sum((f16_t)0.f);
+  return status_from_hip(hipGetLastError());
+}
+
 }  // namespace
 }  // namespace xg
 
@@ -574,7 +590,8 @@ extern "C" int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w
   Prep p{};
   if (int st = fill_rotary(p, rotary, B, S, D, dtype)) return st;
   const bool want_gw = gw_q || gw_k;
-  if (B == 0 || S == 0 || H + Hkv == 0) return XG_OK;
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  if (B == 0 || S == 0 || H + Hkv == 0) return want_gw ? sum_weight_grads(nullptr, 0, 0, D, gw_q, gw_k, w_dtype, st) : XG_OK;
   if (int st = fill_side(p.side[0], q, gq, dq, q_w, H, q_strides, gq_strides, dq_strides, dtype, true)) return st;
   if (int st = fill_side(p.side[1], k, gk, dk, k_w, Hkv, k_strides, gk_strides, dk_strides, dtype, true)) return st;
   if (int st = fill_common(p, B, S, D, eps)) return st;
@@ -589,7 +606,6 @@ extern "C" int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w
   for (Side& sd : p.side) sd.chunks = (sd.H + kBwdHeads - 1) / kBwdHeads;
   p.units = (uint32_t)(B * S);  // tokens: the units of a side follow from its heads
   p.blocks0 = n0;
-  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   const dim3 grid(n0 + n1), block(256);
   auto go = [&](auto full) {
     constexpr bool FULL = decltype(full)::value;
@@ -602,17 +618,5 @@ extern "C" int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w
   };
   p.half_off ? go(std::true_type{}) : go(std::false_type{});
   if (hipGetLastError() != hipSuccess) return XG_ERR_LAUNCH;
-  if (!want_gw) return XG_OK;
-  const dim3 sum_grid((unsigned)(D / 16), 2);
-  auto sum = [&](auto zero) {
-    typedef decltype(zero) WT;
-    hipLaunchKernelGGL((gw_sum_kernel<WT>), sum_grid, dim3(1024), 0, st, workspace, n0, n1, (int)D, (WT*)gw_q, (WT*)gw_k);
-  };
-  if (w_dtype == XG_F32)
-    sum(0.f);
-  else if (w_dtype == XG_BF16)
-    sum((bf16_t)0.f);
-  else
-    sum((f16_t)0.f);
-  return status_from_hip(hipGetLastError());
+  return want_gw ? sum_weight_grads(workspace, n0, n1, D, gw_q, gw_k, w_dtype, st) : XG_OK;
 }
