@@ -500,3 +500,21 @@ def test_the_entry_point_sums_weight_gradients_over_no_rows(device, w_dtype, B, 
         assert rc == 0
         for x, wanted in zip(both, gws):
             assert (x == (0 if wanted is not None else 7)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("w_types", [(torch.float64, torch.float64), (torch.float64, None), (torch.float16, torch.float64)])
+def test_weights_of_other_types_have_gradients_of_their_own_type(device, dtype, w_types):
+    """The kernels read such weights as fp32, forward and backward: the gradient is the fp32 one, in the weight's type."""
+    q, k = make(2, 4, 19, 64, dtype, device, 1), make(2, 2, 19, 64, dtype, device, 2)
+    gq, gk = make(2, 4, 19, 64, dtype, device, 3), make(2, 2, 19, 64, dtype, device, 4)
+    ws = [(1 + 0.2 * torch.randn(64, device=device)).to(t).requires_grad_() if t else None for t in w_types]
+    wf = [w.detach().float() if w is not None else None for w in ws]
+    turn = (*tables(19, 32, device, torch.float32, 1, False), None, [], False, 1e-6)
+    out = _ops().qk_norm_rope(q, k, *ws, *turn)
+    assert all(torch.equal(a, b) for a, b in zip(out, _ops().qk_norm_rope(q, k, *wf, *turn)))
+    want = _ops().qk_norm_rope_bwd(q, k, *wf, gq, gk, *turn, True)
+    there = [i for i, w in enumerate(ws) if w is not None]
+    got = torch.autograd.grad(out, [ws[i] for i in there], (gq, gk), allow_unused=True)
+    for i, gw in zip(there, got):
+        assert gw.dtype == ws[i].dtype and torch.equal(gw, want[2 + i].to(gw.dtype))

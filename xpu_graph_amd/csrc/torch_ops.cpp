@@ -240,9 +240,9 @@ void check_qk(const Tensor& q, const Tensor& k, const OptTensor& wq, const OptTe
 // The weights as the kernels read them: both in the tensors' dtype or both in fp32.
 struct Weights {
   OptTensor q, k;
+  at::ScalarType type;
   int dtype;
-  Weights(const Tensor& x, const OptTensor& wq, const OptTensor& wk) {
-    auto type = x.scalar_type();
+  Weights(const Tensor& x, const OptTensor& wq, const OptTensor& wk) : type(x.scalar_type()) {
     for (const OptTensor* w : {&wq, &wk})
       if (has(*w) && (*w)->scalar_type() != x.scalar_type()) type = at::kFloat;
     auto prepare = [&](const OptTensor& w) -> OptTensor {
@@ -290,8 +290,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rope_bwd(const Tensor& q_in, 
   const Tensor q = operand(q_in), k = operand(k_in), gq = operand(gq_in), gk = operand(gk_in);
   const Weights w(q, wq, wk);
   const int64_t B = q.size(0), H = q.size(1), Hkv = k.size(1), S = q.size(2), D = q.size(3);
-  // a gradient in a weight's own dtype, where the kernel works in fp32 because the other weight does
-  auto kernel_grad = [&](const Tensor& g) { return g.numel() && code(g.scalar_type()) != w.dtype ? at::empty(g.sizes(), g.options().dtype(at::kFloat)) : g; };
+  // a gradient in a weight's own dtype (any that converts), where the kernel works in fp32 because of it or of the other weight
+  auto kernel_grad = [&](const Tensor& g) { return g.numel() && g.scalar_type() != w.type ? at::empty(g.sizes(), g.options().dtype(w.type)) : g; };
   const Tensor kq = kernel_grad(gwq), kk = kernel_grad(gwk);
   const bool any = gwq.numel() || gwk.numel();
   const int64_t n = any ? xg_qk_norm_rope_bwd_workspace_floats(B, H, Hkv, S, D) : 0;
