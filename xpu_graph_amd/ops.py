@@ -1414,13 +1414,18 @@ for _name, _meta in _NATIVE.items():
 
 
 def _load_native_ops():
-    """Their GPU implementations and gradients; without the library a call says how to build it."""
+    """Their GPU implementations and gradients; without the library, or with one that does not fit the installed torch, a call says
+    how to build it.  The ops above do not depend on it."""
+    reason = "is missing"
     if _lib.torch_ops_built():
-        torch.ops.load_library(_lib.TORCH_OPS_PATH)
-        return
+        try:
+            torch.ops.load_library(_lib.TORCH_OPS_PATH)
+            return
+        except OSError as e:  # an unresolved symbol, a file that is no library: nothing of it has been registered
+            reason = f"cannot be loaded ({e})"
 
     def missing(*args, **kwargs):
-        raise ImportError(f"{_lib.TORCH_OPS_PATH} is missing: the mi355x target has no fallback path. Build it with `python -m xpu_graph_amd.build`.")
+        raise ImportError(f"{_lib.TORCH_OPS_PATH} {reason}: the mi355x target has no fallback path. Build it with `python -m xpu_graph_amd.build`.")
 
     for name in _NATIVE:
         _library.impl(name, missing, "CUDA")
