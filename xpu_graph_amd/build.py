@@ -45,6 +45,15 @@ def sources():
     return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def host_compiler():
+    """g++, or the clang++ that hipcc itself runs: what builds the kernels builds the torch ops."""
+    clang = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "clang++")
+    for cand in (shutil.which("g++"), shutil.which("clang++"), clang):
+        if cand and os.path.exists(cand):
+            return cand
+    raise RuntimeError("no host C++ compiler found for torch_ops.cpp")
+
+
 def _compile_torch_ops():
     """Object file of csrc/torch_ops.cpp: host code against the headers of the installed torch."""
     import torch
@@ -53,13 +62,13 @@ def _compile_torch_ops():
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
     obj = os.path.join(OBJ_DIR, "torch_ops.host.o")
     cmd = [
-        shutil.which("g++") or "g++", "-std=c++17", "-O2", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+        host_compiler(), "-std=c++17", "-O2", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root}", f"-I{os.path.join(root, 'torch/csrc/api/include')}",
         f"-I{os.path.join(rocm, 'include')}", "-c", os.path.join(CSRC, "torch_ops.cpp"), "-o", obj,
     ]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed for torch_ops.cpp:\n{proc.stderr}")
+        raise RuntimeError(f"the host compiler failed for torch_ops.cpp:\n{proc.stderr}")
     return obj
 
 
@@ -68,7 +77,7 @@ def _link_torch_ops(obj):
 
     tmp = TORCH_OPS_PATH + ".tmp"
     cmd = [
-        shutil.which("g++") or "g++", "-shared", "-o", tmp, obj, f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-ltorch_cpu", "-ltorch", "-lc10",
+        host_compiler(), "-shared", "-o", tmp, obj, f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-ltorch_cpu", "-ltorch", "-lc10",
         "-lc10_hip", f"-L{_HERE}", "-l:libxpu_graph_amd.so", "-Wl,-rpath,$ORIGIN",
     ]
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -87,7 +96,10 @@ def _compile_one(src):
 
 
 def build_library(verbose=True, jobs=None):
-    """Compile every kernel source for gfx950 and link the C-ABI shared library."""
+    """Compile every kernel source for gfx950 and link the C-ABI shared library, then the torch ops on top of it.
+
+    The kernel library does not depend on the torch half: where that cannot be built (no headers, an error in it) the kernel
+    library is in place all the same when the error is raised, without a torch half of another build beside it."""
     os.makedirs(OBJ_DIR, exist_ok=True)
     srcs = sources()
     wanted = {os.path.basename(s)[:-4] + ".o" for s in srcs} | {"torch_ops.host.o"}
@@ -99,14 +111,18 @@ def build_library(verbose=True, jobs=None):
     with concurrent.futures.ThreadPoolExecutor(max_workers=jobs) as ex:
         torch_obj = ex.submit(_compile_torch_ops)
         objs = list(ex.map(_compile_one, srcs))
-        torch_obj = torch_obj.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [hipcc_path(), "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", tmp, *objs]
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"link failed:\n{proc.stderr}")
     os.replace(tmp, LIB_PATH)
-    _link_torch_ops(torch_obj)
+    try:
+        _link_torch_ops(torch_obj.result())
+    except (RuntimeError, OSError, ImportError) as e:
+        if os.path.exists(TORCH_OPS_PATH):
+            os.remove(TORCH_OPS_PATH)
+        raise RuntimeError(f"{LIB_PATH} is built, the torch ops on top of it are not (their calls raise ImportError): {e}") from e
     if verbose:
         print(f"[xpu_graph_amd.build] wrote {LIB_PATH} and {TORCH_OPS_PATH}", flush=True)
     return LIB_PATH
