@@ -509,10 +509,12 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  * most 0 in a model (minus infinity: no memory).
  * States are fp32 [B,H,D,D] contiguous (row: k, column: v), 16-byte aligned.
  *   state: before the first token, or NULL (zeros); state_out: after the last,
- *     or NULL.  No tokens (S = 0, or a length of 0): state_out is a copy of
- *     state, or zeros, and d_state one of d_state_out; with S = 0 the other
- *     pointers are not looked at, and state results in memory that no kernel
- *     reaches (of the host, or without a device) are left alone.
+ *     or NULL.  state_out may be state, but not overlap it otherwise; d_state may
+ *     overlap neither state nor d_state_out.
+ *   No tokens (S = 0, or a length of 0): state_out is a copy of state, or zeros,
+ *     and d_state one of d_state_out.  With S = 0 only these are looked at, the
+ *     two may be one, and results in memory that no kernel reaches (of the host,
+ *     or without a device) are left alone.
  *   lengths: NULL, or DEVICE int32 / int64 [B] (lengths_64bit), clamped to
  *     [0, S]: tokens from there on are not read, do not reach the state, and
  *     give zeros in out and in the gradients.

@@ -644,3 +644,19 @@ def test_key_heads_without_query_heads_get_zero_gradients(device, dtype):
     assert bwd(dk, dv) == 0
     for x in (dk, dv):
         assert (x[:, :Hkv] == 0).all() and (x[:, Hkv:] == 7).all()
+
+
+@pytest.mark.parametrize("B,H,S", [(1, 3, 40), (1, 3, 700), (2, 64, 300)])
+def test_the_state_of_the_entry_point_in_place(device, B, H, S):
+    """state_out may be state: uncut heads, segments, and an entry of no tokens."""
+    D = 64
+    lib = _xops()._lib.lib()
+    q, k, v = (make((B, H, S, D), torch.bfloat16, device, i, "bhsd") for i in range(3))
+    g, s0 = decays(H, device, "model"), torch.randn(B, H, D, D, device=device)
+    st, n = tuple(q.stride()[:3]), lib.xg_linear_attn_workspace_floats(B, H, S, D)
+    ws = torch.empty(max(n, 1), device=device)
+    for lengths in (None, torch.full((B,), S // 2, device=device), torch.zeros(B, dtype=torch.long, device=device)):
+        want = _ops().linear_attn(q, k, v, g, s0, lengths, 0.1)
+        out, state = torch.empty_like(q), s0.clone()
+        assert entry("xg_linear_attn", q, k, v, g, state, lengths, 1, out, state, ws, n, B, H, H, S, D, st, st, st, st, 0.1, 2) == 0
+        assert torch.equal(out, want[0]) and torch.equal(state, want[1])

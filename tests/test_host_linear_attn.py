@@ -123,3 +123,29 @@ def test_key_heads_without_query_heads():
     assert bwd(B=0) == 0 and bwd(S=0) == 0 and bwd(Hkv=0) == 0  # nothing to write
     assert bwd(dk=None) == -4 and bwd(dv=None) == -4 and bwd(dk=off) == -3 and bwd(s=None) == -4
     assert bwd(D=96) == -2 and bwd(Hkv=1 << 40) == -5 and bwd(s=(ctypes.c_int64 * 3)(1, 2, 3)) == -3
+
+
+def test_states_that_share_memory_are_refused():
+    """Workgroups of one launch read the states that come in while others write the one that goes out."""
+    lib = _lib.lib()
+    B, H, S, D = 1, 2, 64, 64
+    buf = ctypes.create_string_buffer(1 << 17)
+    base = (ctypes.addressof(buf) + 15) & ~15
+    p = ctypes.c_void_p(base)
+    at = lambda floats: ctypes.c_void_p(base + 4 * floats)  # noqa: E731
+    half, whole = D * D, H * D * D
+
+    short = (ctypes.c_int64 * 3)(1 << 14, 1 << 12, 4)  # what passes the states is refused for its strides
+
+    def fwd(state, state_out, S=S):
+        return lib.xg_linear_attn(p, p, p, p, state, None, 0, p, state_out, None, 0, B, H, H, S, D, *[short] * 4, 1.0, 2, None)
+
+    def bwd(state, d_state_out, d_state, S=S):
+        return lib.xg_linear_attn_bwd(p, p, p, p, state, None, 0, p, d_state_out, p, p, p, d_state, None, 0, B, H, H, S, D, *[short] * 7, 1.0, 2, None)
+
+    assert fwd(p, p) == -3 and fwd(p, at(whole)) == -3 and fwd(at(whole), p) == -3 and fwd(None, p) == -3 and fwd(p, None) == -3
+    for n in (S, 0):
+        assert fwd(p, at(half), n) == -7 and fwd(at(half), p, n) == -7 and bwd(None, p, at(half), n) == -7
+    assert bwd(p, None, p) == -7 and bwd(None, p, p) == -7 and bwd(at(half), None, p) == -7
+    assert bwd(p, p, at(whole)) == -3 and bwd(p, p, None) == -3 and bwd(None, None, p) == -3
+    assert bwd(None, p, p, 0) == 0 and bwd(p, None, None, 0) == 0  # nothing is computed: the gradient is where it belongs

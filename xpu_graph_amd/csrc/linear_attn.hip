@@ -829,6 +829,12 @@ int fill(Operand& o, const void* p, const int64_t* s, int group) {
   return fill(o.s, s);
 }
 
+// Whether the states [heads, D, D] at a and b share memory.
+bool states_overlap(const float* a, const float* b, int64_t heads, int64_t D) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b), bytes = (uintptr_t)(heads * D * D) * 4;
+  return a && b && (x < y ? y - x : x - y) < bytes;
+}
+
 // Whether a kernel could reach p: not where there is no device, nor in host memory that HIP does not know.
 bool on_gpu(const void* p) {
   hipPointerAttribute_t at;
@@ -841,8 +847,9 @@ bool on_gpu(const void* p) {
 // The state results of a call without tokens.  Such a call refuses no pointer, as it reads nothing through q, k and v; so what it
 // does read and write is looked at first, and left alone where no kernel could reach it.
 int carry_state(const float* from, float* to, int64_t heads, int64_t D, hipStream_t st) {
-  if (!to || from == to || heads == 0) return XG_OK;
+  if (!to || from == to || heads == 0) return XG_OK;  // (in place)
   if (!aligned_to(to, 16) || (from && !aligned_to(from, 16))) return XG_ERR_BAD_ALIGN;
+  if (states_overlap(from, to, heads, D)) return XG_ERR_BAD_ARG;
   if (!on_gpu(to) || (from && !on_gpu(from))) return XG_OK;
   const int64_t n = heads * D * D / 4, blocks = (n + 255) / 256;
   hipLaunchKernelGGL(carry_state_kernel, dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, st, reinterpret_cast<const f32x4*>(from),
@@ -899,6 +906,8 @@ extern "C" int xg_linear_attn(const void* q, const void* k, const void* v, const
   if (!aligned_to(out, 16) || !aligned_to(log_decay, 4) || (state && !aligned_to(state, 16)) || (state_out && !aligned_to(state_out, 16)) ||
       (workspace && !aligned_to(workspace, 16)) || (lengths && !aligned_to(lengths, lengths_64bit ? 8 : 4)))
     return XG_ERR_BAD_ALIGN;
+  // in place, each thread writes what it has read; shifted, a head's results would land in another's initial state
+  if (state != state_out && states_overlap(state, state_out, B * H, D)) return XG_ERR_BAD_ARG;
   Params p{};
   const int group = (int)(H / Hkv);
   if (int rc = fill(p.pr[0].q, q, q_strides, 1)) return rc;
@@ -965,6 +974,8 @@ extern "C" int xg_linear_attn_bwd(const void* q, const void* k, const void* v, c
                         (const void*)workspace})
     if (t && !aligned_to(t, 16)) return XG_ERR_BAD_ALIGN;
   if (!aligned_to(log_decay, 4) || (lengths && !aligned_to(lengths, lengths_64bit ? 8 : 4))) return XG_ERR_BAD_ALIGN;
+  // dq's workgroups read state and dk's read d_state_out while dv's write d_state
+  if (states_overlap(state, d_state, B * H, D) || states_overlap(d_state_out, d_state, B * H, D)) return XG_ERR_BAD_ARG;
   Params p{};
   const int group = (int)(H / Hkv);
   Operand oq, ok, ov, og;
