@@ -518,9 +518,9 @@ int xg_qk_norm_rope_bwd(const void* q, const void* k, const void* q_w, const voi
  *   lengths: NULL, or DEVICE int32 / int64 [B] (lengths_64bit), clamped to
  *     [0, S]: tokens from there on are not read, do not reach the state, and
  *     give zeros in out and in the gradients.
- *   A NaN or an infinity in q, k or v reaches the outputs of its own chunk of
- *   32 tokens, before it too, and those of later tokens, at least while its
- *   decayed weight is not zero in fp32.
+ *   A NaN or an infinity in q, k or v reaches its own token's output and those
+ *   of later tokens, at least while its decayed weight is not zero in fp32 (an
+ *   infinity may arrive as NaN), and no others; the gradients likewise.
  * xg_linear_attn: a whole sequence, 32 tokens at a time on the matrix cores.
  *   Up to three launches; workspace: xg_linear_attn_workspace_floats fp32 (0:
  *   none needed).

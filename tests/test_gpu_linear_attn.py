@@ -660,3 +660,53 @@ def test_the_state_of_the_entry_point_in_place(device, B, H, S):
         out, state = torch.empty_like(q), s0.clone()
         assert entry("xg_linear_attn", q, k, v, g, state, lengths, 1, out, state, ws, n, B, H, H, S, D, st, st, st, st, 0.1, 2) == 0
         assert torch.equal(out, want[0]) and torch.equal(state, want[1])
+
+
+# what one bad element at token j of an operand reaches: its own row ("row"), the rows of the tokens from j on or up to j, whole
+# ("rows") or in its own column ("col"); of a state its row or column
+REACH = {
+    "q": {"o": "row", "dk": "col up to", "dv": "rows up to", "d_state": "row"},
+    "k": {"o": "rows from", "state": "row", "dq": "col from", "dv": "row"},
+    "v": {"o": "col from", "state": "col", "dq": "rows from", "dk": "row"},
+    "go": {"dq": "row", "dk": "rows up to", "dv": "col up to", "d_state": "col"},
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S,D,j", [(75, 64, 5), (75, 128, 40), (75, 64, 74), (64, 128, 63), (1, 64, 0), (700, 64, 300), (700, 128, 681)])
+@pytest.mark.parametrize("what", list(REACH))
+def test_a_bad_token_reaches_only_what_depends_on_it(device, dtype, S, D, j, what):
+    """The recurrence is causal: a NaN or an infinity at token j leaves the outputs of earlier tokens (the gradients of later ones)
+    and of other columns, heads and batch entries as they are without it."""
+    B, H, Hkv, scale = 2, 4, 2, 0.1
+    group = H // Hkv
+    g = torch.tensor([-0.01, 0.0, -0.2, -0.003], device=device)
+    clean = {n: make((B, h, S, D), dtype, device, 1 + i) for i, (n, h) in enumerate((("q", H), ("k", Hkv), ("v", Hkv), ("go", H)))}
+    gen = torch.Generator().manual_seed(9)
+    s0, ds = (torch.randn(B, H, D, D, generator=gen).to(device) for _ in range(2))
+    b, head, col = 1, (2 if what in ("q", "go") else 1), 11
+    clean[what][b, head, j, col] = 0.0
+    want = reference(clean["q"], clean["k"], clean["v"], g, s0, None, scale, clean["go"], ds)
+    hk = head // group if what in ("q", "go") else head
+    heads = [head] if what in ("q", "go") else list(range(hk * group, hk * group + group))  # the query heads that it meets
+    t = torch.arange(S, device=device)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        x = {n: y.clone() for n, y in clean.items()}
+        x[what][b, head, j, col] = bad
+        o, s = _ops().linear_attn(x["q"], x["k"], x["v"], g, s0, None, scale)
+        dq, dk, dv, d0 = _ops().linear_attn_bwd(x["q"], x["k"], x["v"], g, s0, None, x["go"], ds, scale, True)
+        for name, got in (("o", o), ("state", s), ("dq", dq), ("dk", dk), ("dv", dv), ("d_state", d0)):
+            hurt = torch.zeros(got.shape, dtype=torch.bool, device=device)
+            how = REACH[what].get(name)
+            if how is not None:
+                where = [hk] if name in ("dk", "dv") else heads
+                if name in ("state", "d_state"):
+                    at = (col, slice(None)) if how == "row" else (slice(None), col)
+                    hurt[b, where, at[0], at[1]] = True
+                else:
+                    rows = t == j if how == "row" else (t >= j if how.endswith("from") else t <= j)
+                    cols = torch.arange(D, device=device) == col if how.startswith("col") else torch.ones(D, dtype=torch.bool, device=device)
+                    hurt[b, where] = rows[:, None] & cols
+            label = f"{name} with {bad} in {what}"
+            assert not torch.isfinite(got[hurt]).any(), label
+            check(label, torch.where(hurt, want[name][0].to(got.dtype), got), *want[name], S, g)

@@ -31,6 +31,10 @@
 // A few heads do not fill the chip.  The tokens are then cut into segments: one launch sums up each segment's own state, one
 // turns them into the states before each segment (elementwise, in order), and the kernel above runs all segments at once.
 //
+// The recurrence is causal, and so is the kernel where values are not finite: a chunk whose O shows one is made again token by token.
+// Looking for it costs ten instructions a chunk (bf16 D128 H32: B4 S2048 forward 96.7 -> 99.2 us, backward 163.5 -> 164.3, B8 S4096
+// 238 -> 248 and 577 -> 581, B1 S32768 no change).
+//
 // What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 270 others a chunk), of
 // which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 238 us (1.07 GB, 4.5 TB/s), B8 S2048
 // 122 us, B4 S2048 98 us, B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
@@ -621,12 +625,51 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       O *= row_f;
 
       // O^T += V^T P^T
+      const f32x16 before = O;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         float x[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = P[8 * t + i] * p_f[8 * t + i];
         O = mma_parts(as_parts<T>(vf[t]), split<OP>(x), O);
+      }
+      float worst = fabsf(O[0]);
+#pragma unroll
+      for (int i = 1; i < 16; ++i) worst = __builtin_elementwise_maximum(worst, fabsf(O[i]));
+      if (__builtin_expect(__any(!(worst < __builtin_inff())), 0)) {
+        // The scores of later tokens are zeros, but zero times a value that is not finite is not zero, and a score that is not finite
+        // does not become zero: here the tokens come one by one, each kept from the rows before it (5 us a chunk)
+        O = before;
+        asm volatile("" : "+v"(P));  // (weighed again: the loop needs the registers)
+#pragma unroll 1
+        for (int j = 0; j < n; ++j) {
+          asm volatile("" ::: "memory");
+          f32x16 with = O;
+          const int slot = (j & 15) - 4 * h;
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j >> 4 != t) continue;
+            float x[8];
+            V8 v = TL::col_frag(at.v_lo + AT + 16 * t * TL::RB, at.v_hi + AT + 16 * t * TL::RB);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bool here = 8 * (i >> 2) + (i & 3) == slot;
+              x[i] = here ? P[8 * t + i] * p_f[8 * t + i] : 0.f;
+              v[i] = here ? v[i] : (T)0.f;
+            }
+            with = mma_parts(as_parts<T>(v), split<OP>(x), with);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) O[i] = l32 < j ? O[i] : with[i];
+        }
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {  // (read again, likewise)
+          vf[t] = TL::col_frag(at.v_lo + AT + 16 * t * TL::RB, at.v_hi + AT + 16 * t * TL::RB);
+#pragma unroll
+          for (int dt = 0; dt < D / 32; ++dt)
+            kc[t][dt] = TL::col_frag(at.k_lo[dt] + AT + 16 * t * TL::RB, at.k_hi[dt] + AT + 16 * t * TL::RB);
+        }
       }
 
       if (l32 < n) {
