@@ -710,3 +710,70 @@ def test_a_bad_token_reaches_only_what_depends_on_it(device, dtype, S, D, j, wha
             label = f"{name} with {bad} in {what}"
             assert not torch.isfinite(got[hurt]).any(), label
             check(label, torch.where(hurt, want[name][0].to(got.dtype), got), *want[name], S, g)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("B,H,Hkv,D", [(64, 8, 2, 64), (33, 8, 8, 64), (16, 9, 3, 128)])
+def test_step_of_many_heads(device, dtype, B, H, Hkv, D):
+    """64 columns a workgroup: from 256 workgroups on."""
+    test_step(device, dtype, B, H, Hkv, D)
+
+
+def state_tolerance(S, D, heads, dtype, x):
+    """What a state is off by, relative to the magnitudes that it sums; 2^-24 is half a step of fp32, what a rounding is off by at most.
+    On the way of a product into it: its weight, a power (one step: 2) and a scale (1), and 2.5 x for its exponent; the weighed value
+    (1), what its three 8-bit parts leave out (1) and the 16 products that one matrix instruction adds (16).  Then, with everything
+    added so far, each chunk of 32: the accumulations of its two k-steps (three products of parts each, five of fp16's two-part keys),
+    one decay (1) and that power's own error (2).  Each segment: one decay (1), its power (2), one addition (1)."""
+    chunks = -(-S // 32)
+    segments = max(_xops()._lib.lib().xg_linear_attn_workspace_floats(1, heads, S, D) // (heads * D * D), 1)
+    accumulations = 6 if dtype == torch.bfloat16 else 10
+    return 2.0**-24 * (5 + 16 + (accumulations + 3) * chunks + 4 * segments + 2.5 * x)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("S,D,H", [(1, 64, 3), (33, 128, 3), (64, 64, 2), (700, 128, 3), (4096, 64, 3), (5000, 128, 160)])
+def test_states_to_the_bound_of_chunks_of_32(device, dtype, S, D, H):
+    """The final state, token by token in 64 bits, against the bound for the chunks and segments that the kernels use."""
+    k, v = (make((1, H, S, D), dtype, device, i) for i in range(2))
+    g = torch.tensor([(0.0, -1e-4, -0.02)[h % 3] for h in range(H)], device=device)
+    _, s = _ops().linear_attn(k, k, v, g, None, None, 0.125)
+    for h in range(0, H, max(1, H // 6)):
+        w = powers(g[h : h + 1], S - 1 - torch.arange(S, device=device))[0][:, None]
+        kd, vd = k[0, h].double(), v[0, h].double()
+        want, mag = (kd * w).T @ vd, (kd.abs() * w).T @ vd.abs()
+        x = min(abs(g[h].item()) * S, 104)
+        tol = state_tolerance(S, D, H, dtype, x) * mag + 1e-37
+        assert ((s[0, h].double() - want).abs() <= tol).all()
+
+
+def test_a_compiled_training_step_of_the_layer(device):
+    """Forward and gradients through the training compiler: the same ops in the same order, so the values are equal."""
+    from xpu_graph_amd import mi355x_compiler
+
+    _xops().enable_autograd()
+    B, S, H, D = 2, 100, 2, 64
+    bf = torch.bfloat16
+    ang = torch.rand(S, D // 2, generator=torch.Generator().manual_seed(0)) * 6
+    cos, sin, g = ang.cos().to(device), ang.sin().to(device), decays(H, device, "model")
+    pos = torch.arange(S, device=device)
+    n = torch.tensor([S, 61], device=device)
+
+    def attend(q, k, v, wq, wk, state):
+        q, k = torch.ops.xpu_ops.qk_norm_rope(q, k, wq, wk, cos, sin, pos, [], False, 1e-6)
+        q = torch.ops.xpu_ops.rope_axes(q, cos, sin, pos, [])
+        return torch.ops.xpu_ops.linear_attn(q, k, v, g, state, n, D**-0.5)
+
+    def inputs(seed):
+        x = [make((B, H, S, D), bf, device, seed + i) for i in range(3)]
+        x += [(1 + 0.1 * torch.randn(D, device=device)).to(bf) for _ in range(2)] + [torch.randn(B, H, D, D, device=device)]
+        return [t.requires_grad_() for t in x]
+
+    step = torch.compile(attend, backend=mi355x_compiler(is_training=True), dynamic=False)
+    for seed in (0, 10):
+        leaves = inputs(seed)
+        up = make((B, H, S, D), bf, device, seed + 7), torch.randn(B, H, D, D, device=device)
+        want, got = attend(*leaves), step(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        want, got = (torch.autograd.grad(y, leaves, up) for y in (want, got))
+        assert all(torch.equal(a, b) for a, b in zip(want, got))

@@ -518,3 +518,22 @@ def test_weights_of_other_types_have_gradients_of_their_own_type(device, dtype, 
     got = torch.autograd.grad(out, [ws[i] for i in there], (gq, gk), allow_unused=True)
     for i, gw in zip(there, got):
         assert gw.dtype == ws[i].dtype and torch.equal(gw, want[2 + i].to(gw.dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("case,S", [(CASES[1], 3001), (CASES[4], 2001), (CASES[6], 2001), (CASES[6], 6001)])
+def test_two_and_four_heads_a_thread_of_the_other_types(device, dtype, case, S):
+    check_qk(device, dtype, case, 2, 9, 3, S, "own")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("case,S", [(CASES[6], 1501), (CASES[6], 6001), (CASES[4], 6001), (CASES[2], 9001)])
+def test_two_and_eight_heads_a_thread_of_the_other_types(device, dtype, case, S):
+    D, R, sections, woven, kind, per, _ = case
+    B, H, P = 2, 11, 70
+    x = make(B, H + 2, S, D, dtype, device, 5)[:, 1:-1]  # a part of something else
+    cos, sin = tables(P if kind != "none" else S, R // 2, device, torch.float32, 2, per == 2)
+    pos = make_positions(kind if kind != "s" else "bs", max(len(sections), 1), B, S, P, device, 3)
+    ang = angles(cos, sin, pos, sections, woven, B, S, R)
+    assert_rounded_once(_ops().rope_axes(x, cos, sin, pos, sections, woven), *turn(x.double(), ang, R), "rope_axes")
+    assert_rounded_once(_ops().rope_axes_bwd(x, cos, sin, pos, sections, woven), *turn_back(x.double(), ang, R), "rope_axes_bwd")
