@@ -32,14 +32,14 @@
 // turns them into the states before each segment (elementwise, in order), and the kernel above runs all segments at once.
 //
 // The recurrence is causal, and so is the kernel where values are not finite: a chunk whose O shows one is made again token by token.
-// Looking for it costs ten instructions a chunk (bf16 D128 H32: B4 S2048 forward 96.7 -> 99.2 us, backward 163.5 -> 164.3, B8 S4096
-// 238 -> 248 and 577 -> 581, B1 S32768 no change).
+// Looking for it costs ten instructions a chunk (bf16 D128 H32, in turn: B4 S2048 forward 96.7 -> 99.2 us, backward 163.5 -> 164.3,
+// B1 S32768 no change; B8 S4096, whose runs scatter between 220 and 250, at most 4 %, backward 577 -> 581).
 //
-// What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 270 others a chunk), of
-// which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 238 us (1.07 GB, 4.5 TB/s), B8 S2048
-// 122 us, B4 S2048 98 us, B1 S32768 332 us (eight: 1.54 GB, 4.6 TB/s); backward B8 S4096
-// 580 us, B4 S2048 160 us (0.67 GB by the counters: dv and dk share all they can; 384 workgroups on 256 compute units), B1 S32768
-// 788 us.
+// What bounds it: memory, and behind it the instructions of a wave (34 to 42 MFMAs of 32 cycles and about 280 others a chunk), of
+// which one alone on its SIMD makes a chunk in 1.4 us.  bf16 D 128 H 32: forward B8 S4096 240 us (1.07 GB, 4.5 TB/s), B8 S2048
+// 125 us, B4 S2048 99 us, B1 S32768 334 us (eight segments: 1.45 GB by the counters, 4.4 TB/s); backward B8 S4096
+// 580 us, B4 S2048 164 us (0.67 GB by the counters: dv and dk share all they can; 384 workgroups on 256 compute units), B1 S32768
+// 790 us.  fp16 runs most products two or three times: forward B4 S2048 212 us, backward B1 H64 S4096 379 us against 169.
 #include "sdpa_common.hpp"
 
 namespace xg {
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void group_sum_kernel(const GroupSum p) {
 }
 
 // One token: the state of a head is read, updated and written in place, and the row q S comes out of the same pass.
-// Bound by the state's bytes (two ways): B64 H32 D128 47 us, 268 MB, 5.7 TB/s on fresh states; one sequence 3.0 us.  A workgroup
+// Bound by the state's bytes (two ways): B64 H32 D128 45.4 us, 268 MB, 5.9 TB/s on fresh states; one sequence 3.0 us.  A workgroup
 // takes W columns of one head's state, 16 bytes a lane, with streamed loads and stores (cached ones: 54 us).
 struct StepParams {
   const void* q;
@@ -825,10 +825,17 @@ int64_t chunks_of(int64_t S) { return (S + C - 1) / C; }
 
 // How many segments the tokens of a head are cut into, four chunks at least each.  Cutting reads K and V twice; not cutting leaves
 // the chip idle where there are few heads, each of which takes 1.4 us a chunk.  With fewer than half the heads that fill it with
-// one wave a SIMD they are cut to fill it once, or twice where that would be less than four segments.  Measured (bf16 D 128, us,
-// uncut / segments: once, twice the chip): forward 32 heads S 32768 1362 / 8: 336, 16: 356; 64 heads S 8192 348 / 4: 181, 8: 180; 96
-// heads S 4096 176 / 2: 154, 5: 137; 128 heads S 2048 98 / 2: 98, 4: 102; 192 heads 109 / 2: 132; backward (three times the heads)
-// 32 heads S 32768 1242 / 2: 1007, 5: 790, 64 heads S 8192 358 / 4: 394.
+// one wave a SIMD they are cut to fill it once, or twice where that would be less than four segments.  Measured (us; uncut /
+// segments: to fill the chip once, twice).  bf16 D 128 forward: 32 heads S 32768 1362 / 8: 336, 16: 356; 64 heads S 4096 179 / 4: 97,
+// 8: 102; 96 heads S 4096 185 / 2: 159, 5: 135; 126 heads S 2048 96 / 2: 92, 4: 94; 128 heads S 2048 99 / 2: 98, 4: 100, S 8192
+// 358 / 2: 321, 4: 323; 192 heads S 2048 109 / 2: 132.  Backward (three times the heads) 32 heads S 32768 1242 / 2: 1007, 5: 790, S
+// 4096 158 / 2: 145, 5: 114; 42 heads 159 / 2: 151, 4: 139; 43 heads 161 / 3: 150; 48 heads 165 / 3: 160; 56 heads 167 / 3: 181; 64
+// heads S 8192 358 / 4: 394.  bf16 D 64 forward: 64 heads S 4096 128 / 8: 57, 16: 63; 128 heads S 2048 68 / 4: 56, 8: 62; 192 heads
+// 68 / 2: 83, 5: 75; 252 heads 69 / 2: 90, 4: 92; backward S 2048 64 heads 61 / 2: 76, 5: 61; 80 heads 64 / 2: 83, 4: 77.  So the step at
+// half the chip is right for bf16 within 10 % (D 64 between half of it and a third: up to 25 % too early; D 128 with 128 long heads: 11 %
+// too early).  fp16's chunk costs two to three times the products for the same bytes, so a cut pays for longer there: D 128 128
+// heads S 2048 213 / 4: 161, S 8192 832 / 4: 562, backward 43 heads S 4096 384 / 3: 303; D 64 256 heads 135 / 4: 105, backward 86
+// heads S 2048 200 / 3: 118; the rule does not tell the types apart.
 void segments(int64_t heads, int64_t n_problems, int64_t S, int64_t D, int& n_seg, int& seg_chunks) {
   const int64_t chunks = chunks_of(S), groups = heads * n_problems, full = 256 * (128 / D);
   int64_t n = groups >= full / 2 ? 1 : (full / groups >= 4 ? full : 2 * full) / groups;
@@ -1131,7 +1138,7 @@ extern "C" int xg_linear_attn_step(const void* q, const void* k, const void* v, 
   p.H = (int)H;
   p.group = (int)(H / Hkv);
   p.scale = scale;
-  // 64 columns a workgroup (B64 H32 D128 47 us; 32: 49, 128: 49), 32 where those are too few to give every compute unit one
+  // 64 columns a workgroup (B64 H32 D128, replayed from a graph, 47 us; 32: 49, 128: 49; D64 12.9), 32 where those are too few to give every compute unit one
   // (B1 H32 3.5 us with 64, 3.0 with 32; B8 H32 7.5 and 7.9)
   const bool wide = B * H * (D / 64) >= 256;
   const dim3 grid((unsigned)(B * H * (D / (wide ? 64 : 32))));

@@ -19,8 +19,9 @@
 // Measured on fresh inputs (bf16, D 128): rope_axes B2 S6144 H32, three axes 39 us, 201 MB, 5.1 TB/s; qk_norm_rope B4 S2048 H32/8
 // 32 us, 168 MB, 5.2 TB/s, H32/32 51 us, 268 MB, 5.3 TB/s, its backward with the sum of the weight gradients 78 us, 403 MB, 5.1 TB/s
 // (a copy of that size: 6.3).  Loads behind a condition each cost a quarter (47, 45, 72, 93 us), cached loads and results that
-// lie head by head where the inputs lie token by token a tenth more.  D 96 leaves two of a row's eight lanes idle: fp16 B3 S1371
-// H10/5 13 us forward, 18 + 4 us backward.
+// lie head by head where the inputs lie token by token a tenth more.  With three axes and D 96, fp16 B3 S1371 H10/5 takes 10.5 us
+// forward, 19 + 4 us backward: a row leaves two of its eight lanes idle, and each axis' position is read before its table row.
+// fp32 D 128: rope_axes B1 S4096 H32, three axes 41 us, 134 MB, 3.3 TB/s; qk_norm_rope H32/8 42 us, 168 MB, 4.0 TB/s.
 #include "xg_common.hpp"
 
 namespace xg {
@@ -490,10 +491,14 @@ int run_prep(Prep& p, int64_t tokens, int dtype, hipStream_t stream) {
     return launch_prep<float, NORM, FULL, kHeads>(p, tokens, stream);
   };
   // Several heads a thread share one read of the tables and keep more bytes on their way; few rows are spread over as many
-  // threads as there are.  By the threads that one head each would make, bf16 D 128 on fresh inputs, us with one / two / four
-  // (eight) heads a thread: rope_axes, three axes, H32 131 k (S 512) 5.4 / 5.5 / 6.9 (9.0), 524 k 12.4 / 8.9 / 9.1 (10.5), 1.05 M
-  // 20.4 / 17.4 / 14.2 (14.5), 3.1 M - (39); qk_norm_rope H32/8 328 k (S 1024) 6.6 / 6.9 / 8.0, 655 k 11.7 / 9.5 / 10.3, 1.3 M
-  // 19.7 / 18.2 / 16.1, 2.6 M 32 with four, 38 with eight (registers).
+  // threads as there are.  By the threads that one head each would make, on fresh inputs, us with one / two / four (eight) heads a
+  // thread.  bf16 D 128: rope_axes, three axes, H32 131 k (S 512) 5.3 / 5.5 / 6.8 (9.0), 262 k 7.2 / 6.4 / 7.2 (9.1), 524 k 12.5 / 8.8 / 9.1
+  // (10.2), 1.05 M 20.2 / 17.6 / 14.0 (14.1), 3.1 M - (39); qk_norm_rope H32/8 328 k (S 1024) 6.7 / 6.9 / 8.0, 655 k 12.3 / 9.6 / 10.2,
+  // 1.3 M 20.1 / 18.1 / 16.5, 2.6 M 38.7 / 34.5 / 32.4 (38, registers).  fp16, D 64 and D 96 with three axes: the same within 5 % (D 96 fp16
+  // qk_norm_rope 655 k 15.3 / 10.7 / 11.8, 1.3 M 26.6 / 20.7 / 16.2; rope_axes 1.05 M 19.8 / 16.2 / 13.1 (13.8)).  fp32 moves twice the
+  // bytes a head and wants two at the most, which the rule does not tell: D 128 qk_norm_rope 328 k 12.3 / 11.3 / 13.7, 655 k 21.2 / 20.0 /
+  // 19.0, 1.3 M 38.5 / 37.8 / 41.9, 2.6 M 74 / 73 / 81; rope_axes 524 k 18.8 / 17.7 / 17.7 (23.4), 1.05 M 32.6 / 31.8 / 36.6 (41.1), 2.1 M
+  // 60 / 58 / 63 (75); D 96 rope_axes 2.1 M 57 / 52 / 48 (53).
   const int64_t threads = (tokens * (p.side[0].H + p.side[1].H)) << p.tpr_log2;
   auto with = [&](auto heads) { return p.half_off ? go(std::true_type{}, heads) : go(std::false_type{}, heads); };
   constexpr int kMany = NORM ? 4 : 8;
