@@ -638,7 +638,8 @@ __global__ __launch_bounds__(D * 2) __attribute__((amdgpu_waves_per_eu(2, 2))) v
       for (int i = 1; i < 16; ++i) worst = __builtin_elementwise_maximum(worst, fabsf(O[i]));
       if (__builtin_expect(__any(!(worst < __builtin_inff())), 0)) {
         // The scores of later tokens are zeros, but zero times a value that is not finite is not zero, and a score that is not finite
-        // does not become zero: here the tokens come one by one, each kept from the rows before it (5 us a chunk)
+        // does not become zero: here the tokens come one by one, each kept from the rows before it (9 us a
+        // chunk more, 12 in fp16, also in those after it, whose state holds the value)
         O = before;
         asm volatile("" : "+v"(P));  // (weighed again: the loop needs the registers)
 #pragma unroll 1
